@@ -59,9 +59,8 @@ __device__ __forceinline__ float gelu_f(float x) {
   const float q1 = fmaf(t, c, 1.f);
   return fmaf(-a, __builtin_amdgcn_exp2f(-q1), fmaxf(x, 0.f));
 }
-// the same function of TWO values at once (round 6): the polynomial and the final fma as packed fp32 operations (v_pk_fma_f32: two
-// per lane per issue slot; the GEGLU epilogue of a K = 320 launch is ~85 us of VALU issue out of 282 us); every operation is the
-// scalar one per component, so the results are bit-identical to gelu_f
+// the same function of TWO values at once: every operation is the scalar one per component, so the results are bit-identical to
+// gelu_f (the build switches the packed fp32 instructions off, so hipcc emits scalar ones)
 typedef float fdmi_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ fdmi_f2 gelu_f2(fdmi_f2 x) {
   const fdmi_f2 a = {fabsf(x.x), fabsf(x.y)};

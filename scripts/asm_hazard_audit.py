@@ -155,7 +155,7 @@ def main():
     a = ap.parse_args()
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
-        subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "--cuda-device-only", "-S", "-o", out,
+        subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-S", "-o", out,
                         os.path.abspath(a.source)], check=True, stderr=subprocess.DEVNULL,
                        cwd=os.path.dirname(os.path.abspath(a.source)))
         text = open(out).read()

@@ -16,7 +16,7 @@ for o in "$src"/*.o; do
 done
 for f in "$@"; do
   b=$(basename "$f" .hip)
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result $flags -c "$src/$f" -o "$dst/$b.o" &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops $flags -c "$src/$f" -o "$dst/$b.o" &
 done
 wait
 for f in "$@"; do objs="$objs $dst/$(basename "$f" .hip).o"; done

@@ -13,6 +13,7 @@ def main():
     src = sys.argv[1]
     flt = sys.argv[2] if len(sys.argv) > 2 else ""
     out = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result",
+                          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                           "-Rpass-analysis=kernel-resource-usage", "-I", CSRC, "-c", src, "-o", "/dev/null"],
                          capture_output=True, text=True).stderr
     cur, rows = None, {}

@@ -50,6 +50,6 @@ python scripts/rocprof_to_profiles.py --round "$round" --steps 4 --stats-dir "$o
 find "$out" -name '*kernel_trace.csv' -delete; find "$out" -name '*counter_collection.csv' -delete
 mkdir -p "$out/profiles" && cp profiles/r${round}_kernel_stats.csv profiles/r${round}_pmc_hbm_traffic.csv profiles/r${round}_traffic.json profiles/r${round}_l2_hit_rate.csv profiles/r${round}_clock.csv "$out/profiles/" 2>/dev/null
 echo "== register-only MFMA rate under full-chip load (scripts/ubench/mfma_rate.hip)"
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -o /tmp/mfma_rate scripts/ubench/mfma_rate.hip && /tmp/mfma_rate > "$out/profiles/r${round}_mfma_rate.txt" 2>&1
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/mfma_rate scripts/ubench/mfma_rate.hip && /tmp/mfma_rate > "$out/profiles/r${round}_mfma_rate.txt" 2>&1
 cat "$out/profiles/r${round}_mfma_rate.txt"
 du -sh "$out"; tail -20 "$out/summary.txt"
