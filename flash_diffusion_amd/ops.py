@@ -6,7 +6,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import GemmDesc, check, lib, ptr, stream_ptr
+from ._lib import Fp8Desc, GemmDesc, check, lib, ptr, stream_ptr
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -411,6 +411,233 @@ def attn_bwd(q, k, v, o, do, lse, H, scale, out=None):
                               ptr(do), do.stride(1), ptr(lse), ptr(dq), dq.stride(1), ptr(dk), dk.stride(1),
                               ptr(dv), dv.stride(1), ptr(ws), B, H, Sq, Skv, d, scale, stream_ptr()))
     return dq, dk, dv
+
+
+# ---- 8-bit products with a scale for each block of 128 (csrc/fp8.hip) -----------------------------------------------------------
+F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _here(t, what):
+    """an operand of the 8-bit / embedding entry points: on the current device (their launches go to its current stream)"""
+    if not (t.is_cuda and t.get_device() == torch.cuda.current_device()):
+        raise ValueError(f"{what} is on {t.device}: it has to be on the current GPU")
+    return t
+
+
+def _rows(t, what, dtypes=(BF16, F32)):
+    """a [M, K] operand whose rows are contiguous -> its row stride"""
+    _here(t, what)
+    if t.dim() != 2 or t.dtype not in dtypes:
+        raise ValueError(f"{what}: need a 2-D tensor of {dtypes}, got {tuple(t.shape)} {t.dtype}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: the last dimension has to be contiguous")
+    if t.shape[0] > 1:
+        if t.stride(0) < t.shape[1]:
+            raise ValueError(f"{what}: rows overlap (stride {t.stride(0)} < {t.shape[1]})")
+        return t.stride(0)
+    return t.shape[1]
+
+
+def _pad(n, to):
+    return -(-n // to) * to
+
+
+class Fp8Rows:
+    """Rows of activations in 8 bits: codes [M, K padded to 128] e4m3 (zeros behind K), scales [M, K / 128 padded to 4] e8m0, one for
+    each 128 columns.  The value of a code is code * scale; .values() gives them as [M, K]."""
+
+    def __init__(self, M, K, device):
+        self.M, self.K, self.Kp, self.Ks = M, K, _pad(K, 128), _pad(_pad(K, 128) // 128, 4)
+        self.codes = torch.empty(M, self.Kp, dtype=F8, device=device)
+        self.scales = torch.empty(M, self.Ks, dtype=E8, device=device)
+
+    def values(self, dtype=F32):
+        """read back (a test / debugging aid in torch operations; e4m3 times a power of two is exact in bf16 and fp32)"""
+        c = self.codes.float().view(self.M, self.Kp // 128, 128) * self.scales[:, :self.Kp // 128].float()[..., None]
+        return c.view(self.M, self.Kp)[:, :self.K].to(dtype)
+
+
+class Fp8Weight:
+    """A frozen weight [N, K] in 8 bits: codes [N, K padded to 128], scales [ceil(N / 128), K / 128 padded to 4], one for each 128 x 128
+    block; codes_t / scales_t (or None): the transpose, which gemm_fp8_dgrad contracts with."""
+
+    def __init__(self, N, K, device, transposed):
+        self.N, self.K, self.Kp, self.Np = N, K, _pad(K, 128), _pad(N, 128)
+        # (scale rows are padded to 4: the padding is never read as a scale, but initialised memory is easier to look at)
+        self.codes = torch.empty(N, self.Kp, dtype=F8, device=device)
+        self.scales = torch.zeros(self.Np // 128, _pad(self.Kp // 128, 4), dtype=torch.uint8, device=device).view(E8)
+        self.codes_t = self.scales_t = None
+        if transposed:
+            self.codes_t = torch.empty(K, self.Np, dtype=F8, device=device)
+            self.scales_t = torch.zeros(self.Kp // 128, _pad(self.Np // 128, 4), dtype=torch.uint8, device=device).view(E8)
+
+    def values(self, dtype=F32):
+        s = self.scales[:, :self.Kp // 128].float().repeat_interleave(128, 0)[:self.N].repeat_interleave(128, 1)
+        return (self.codes.float() * s)[:, :self.K].to(dtype)
+
+
+def pack_weight_fp8(w, transposed=False):
+    """w [N, K] f32 / bf16 -> Fp8Weight (once per weight); transposed: keep the codes of w^T too, for gemm_fp8_dgrad"""
+    ld = _rows(w, "weight")
+    if w.shape[0] < 1 or w.shape[1] < 1:
+        raise ValueError(f"weight is empty: {tuple(w.shape)}")
+    o = Fp8Weight(w.shape[0], w.shape[1], w.device, transposed)
+    check(lib().fdmi_pack_fp8(ptr(w), int(w.dtype == F32), ld, o.N, o.K, ptr(o.codes), o.Kp, ptr(o.scales), o.scales.stride(0),
+                              ptr(o.codes_t), o.Np, ptr(o.scales_t), 0 if o.scales_t is None else o.scales_t.stride(0), stream_ptr()))
+    return o
+
+
+def quant_fp8(x):
+    """x [M, K] bf16 / f32 -> Fp8Rows"""
+    return rmsnorm_fp8(x, None, 0.0)
+
+
+def rmsnorm_fp8(x, w, eps):
+    """x * rsqrt(mean(x^2) + eps) * w (T5LayerNorm, computed in fp32), quantised -> Fp8Rows; w [K] f32 (None: x itself)"""
+    ld = _rows(x, "x")
+    if x.shape[1] < 1:
+        raise ValueError(f"x has no columns: {tuple(x.shape)}")
+    if w is not None:
+        _here(w, "w")
+        if w.dtype != F32 or tuple(w.shape) != (x.shape[1],) or not w.is_contiguous():
+            raise ValueError(f"w: need a contiguous fp32 [{x.shape[1]}], got {tuple(w.shape)} {w.dtype}")
+    o = Fp8Rows(x.shape[0], x.shape[1], x.device)
+    check(lib().fdmi_quant_fp8(ptr(x), int(x.dtype == F32), ld, ptr(w), eps, ptr(o.codes), o.Kp, ptr(o.scales), o.Ks, o.M, o.K,
+                               stream_ptr()))
+    return o
+
+
+def _fp8_operands(d, A, K, what):
+    """fills the activation side of a descriptor from Fp8Rows or from [M, K] bf16 / f32 rows (quantised by the call itself); returns
+    (M, device, what has to stay alive until the launch)"""
+    if isinstance(A, Fp8Rows):
+        if A.K != K:
+            raise ValueError(f"{what} has {A.K} columns, the weight contracts over {K}")
+        _here(A.codes, what)
+        d.M, d.X, d.ldx, d.sx, d.ldsx = A.M, A.codes.data_ptr(), A.Kp, A.scales.data_ptr(), A.Ks
+        return A.M, A.codes.device, A
+    ld = _rows(A, what)
+    M = A.shape[0]
+    if A.shape[1] != K:
+        raise ValueError(f"{what} has {A.shape[1]} columns, the weight contracts over {K}")
+    Kp = _pad(K, 128)
+    Ks = _pad(Kp // 128, 4)
+    scratch = torch.empty(M * (Kp + Ks) + 1, dtype=torch.uint8, device=A.device)
+    d.M, d.x, d.ldxr, d.x_f32 = M, A.data_ptr(), ld, int(A.dtype == F32)
+    d.X, d.ldx, d.sx, d.ldsx = scratch.data_ptr(), Kp, scratch.data_ptr() + M * Kp, Ks
+    return M, A.device, scratch
+
+
+def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what):
+    d = Fp8Desc()
+    d.N, d.K = N, K
+    M, dev, keep = _fp8_operands(d, A, K, what)
+    if out is None:
+        out = torch.empty(M, N, dtype=F32 if out_f32 else BF16, device=dev)
+    elif tuple(out.shape) != (M, N):
+        raise ValueError(f"out: need [{M}, {N}], got {tuple(out.shape)}")
+    d.C, d.ldc, d.out_f32, d.act = out.data_ptr(), _rows(out, "out"), int(out.dtype == F32), act
+    d.W, d.ldw, d.sw, d.ldsw = codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0)
+    _here(codes, "weight")
+    if bias is not None:
+        _here(bias, "bias")
+        if bias.dtype != F32 or tuple(bias.shape) != (N,) or not bias.is_contiguous():
+            raise ValueError(f"bias: need a contiguous fp32 [{N}], got {tuple(bias.shape)} {bias.dtype}")
+        d.bias = bias.data_ptr()
+    if residual is not None:
+        if act != ACT_NONE:
+            raise ValueError("an activation and a residual exclude each other")
+        if tuple(residual.shape) != (M, N):
+            raise ValueError(f"residual: need [{M}, {N}], got {tuple(residual.shape)}")
+        d.residual, d.ldr = residual.data_ptr(), _rows(residual, "residual", (out.dtype,))
+    if M:
+        check(lib().fdmi_gemm_fp8(C.byref(d), stream_ptr()))
+    return out
+
+
+def gemm_fp8(A, W, *, bias=None, residual=None, act=ACT_NONE, out=None, out_f32=False):
+    """act(A W^T + bias) or A W^T + bias + residual with 8-bit operands: A Fp8Rows, or [M, K] bf16 / f32 rows that the call quantises;
+    W Fp8Weight; bias [N] f32; residual and out [M, N] of one type (bf16, or f32 with out_f32).  fp32 sums, one rounding."""
+    return _fp8_product(A, W.K, W.N, W.codes, W.scales, bias, residual, act, out, out_f32, "A")
+
+
+def gemm_fp8_dgrad(dY, W, *, residual=None, out=None, out_f32=False):
+    """dY W: the gradient of gemm_fp8's input, dY [M, N] quantised along N.  W has to be packed with transposed=True"""
+    if W.codes_t is None:
+        raise ValueError("gemm_fp8_dgrad needs pack_weight_fp8(w, transposed=True)")
+    return _fp8_product(dY, W.N, W.K, W.codes_t, W.scales_t, None, residual, ACT_NONE, out, out_f32, "dY")
+
+
+def gated_fp8(A, W, W2):
+    """gelu_tanh(A W^T) * (A W2^T), quantised: the gated feed-forward's first half (T5: wi_0, wi_1) -> Fp8Rows [M, N].  The product is
+    formed in fp32 and never leaves the kernel in any other form than its codes."""
+    if (W.N, W.K) != (W2.N, W2.K):
+        raise ValueError(f"the two weights differ in shape: {(W.N, W.K)} and {(W2.N, W2.K)}")
+    d = Fp8Desc()
+    d.N, d.K = W.N, W.K
+    M, dev, keep = _fp8_operands(d, A, W.K, "A")
+    _here(W.codes, "weight")
+    _here(W2.codes, "second weight")
+    o = Fp8Rows(M, W.N, dev)
+    d.W, d.ldw, d.sw, d.ldsw = W.codes.data_ptr(), W.Kp, W.scales.data_ptr(), W.scales.stride(0)
+    d.W2, d.sw2 = W2.codes.data_ptr(), W2.scales.data_ptr()
+    d.H, d.ldh, d.sh, d.ldsh = o.codes.data_ptr(), o.Kp, o.scales.data_ptr(), o.Ks
+    if M:
+        check(lib().fdmi_gemm_fp8(C.byref(d), stream_ptr()))
+    return o
+
+
+# ---- token embedding (csrc/embed.hip) ------------------------------------------------------------------------------------------
+def _ids(ids):
+    _here(ids, "ids")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids: need int32 or int64, got {ids.dtype}")
+    return ids.contiguous()
+
+
+def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16):
+    """scale * table[ids] (+ pos[t], t the last index of ids) -> [*ids.shape, D] in `dtype`: table [V, D] f32 / bf16, ids int32 / int64,
+    pos [>= ids.shape[-1], D] f32.  An id outside the table gives a row of NaN."""
+    ld = _rows(table, "table")
+    ids = _ids(ids)
+    V, D = table.shape
+    if V < 1 or D < 1 or dtype not in (BF16, F32):
+        raise ValueError(f"table {tuple(table.shape)} -> {dtype}: need rows, columns, and bf16 or fp32 out")
+    S = ids.shape[-1] if ids.dim() else 1
+    ldp = 0
+    if pos is not None:
+        ldp = _rows(pos, "pos", (F32,))
+        if pos.shape[0] < S or pos.shape[1] != D:
+            raise ValueError(f"pos: need at least [{S}, {D}], got {tuple(pos.shape)}")
+    out = torch.empty(*ids.shape, D, dtype=dtype, device=table.device)
+    n = ids.numel()
+    if n:
+        check(lib().fdmi_embed_fwd(ptr(table), int(table.dtype == F32), V, D, ld, ptr(ids), int(ids.dtype == torch.int64), n, scale,
+                                   ptr(pos), S, ldp, ptr(out), int(dtype == F32), stream_ptr()))
+    return out
+
+
+def embed_bwd(dy, ids, V, scale=1.0, out=None):
+    """grad [V, D] f32 of embed_fwd's table: grad[v] = scale * sum of the rows of dy [*ids.shape, D] (bf16 / f32) whose id is v; out:
+    accumulated into (+=) instead of a new gradient.  Sums run in a fixed order (bit-reproducible); ids outside the table are dropped."""
+    ids = _ids(ids)
+    D = dy.shape[-1]
+    if tuple(dy.shape[:-1]) != tuple(ids.shape) or D < 1 or V < 1:
+        raise ValueError(f"dy {tuple(dy.shape)} does not match ids {tuple(ids.shape)} (V = {V})")
+    n = ids.numel()
+    rows = dy.reshape(n, D)
+    ld = _rows(rows, "dy")
+    acc = out is not None
+    if acc:
+        if tuple(out.shape) != (V, D):
+            raise ValueError(f"out: need [{V}, {D}], got {tuple(out.shape)}")
+    else:
+        out = torch.empty(V, D, dtype=F32, device=dy.device)
+    ldg = _rows(out, "out", (F32,))
+    ws = torch.empty(lib().fdmi_embed_bwd_ws_bytes(n, D), dtype=torch.uint8, device=dy.device)
+    check(lib().fdmi_embed_bwd(ptr(rows), int(dy.dtype == F32), ld, ptr(ids), int(ids.dtype == torch.int64), n, V, D, scale, int(acc),
+                               ptr(out), ldg, ptr(ws), stream_ptr()))
+    return out
 
 
 # ---- misc --------------------------------------------------------------------------------------

@@ -206,6 +206,52 @@ int fdmi_dmd_loss(const float* s, const float* noisy, const float* real, const f
                   const float* msig_alpha, const float* kb, float* w, float* grad, float* loss, int B, int64_t per,
                   void* stream);
 
+/* ---------------- 8-bit matrix products with a scale for each block of 128 (csrc/fp8.hip) ----------------
+ * The frozen text encoders' linears (T5-XXL behind embedders/t5/t5_embedder_model.py:11-104) in 8 bits: codes are e4m3, a scale is
+ * a power of two held as its biased exponent in one byte (e8m0), 2^e the smallest power with amax <= 448 2^e over the block.  A row of
+ * activations has one scale per 128 columns, a weight [N][K] one per 128 x 128 block.  Code rows are padded with zeros to a multiple
+ * of 128 columns (leading dimension: a multiple of 128), scale rows to a multiple of four bytes; both start 16- / 4-byte aligned.
+ * An infinity or NaN becomes the NaN code and does not enter its block's scale.
+ *
+ * fdmi_quant_fp8: x [M][K] (bf16, or fp32 when x_f32) -> codes [M][ldq], scales [M][lds].  norm (optional, [K] fp32): quantises
+ * x * rsqrt(mean(x^2) + eps) * norm, computed in fp32 (T5LayerNorm).
+ * fdmi_pack_fp8: a weight [N][K] -> codes [N][ldq], scales [ceil(N/128)][lds] and, when codes_t is given, the transposed codes
+ * codes_t [K][ldqt], scales_t [ceil(K/128)][ldst] (ldqt >= N padded to 128) that an input gradient contracts with.  Padding bytes
+ * of the codes are written; those of the scales are not read.                                                                       */
+int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, void* codes, int64_t ldq, void* scales, int64_t lds,
+                   int64_t M, int K, void* stream);
+int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, int64_t ldq, void* scales, int64_t lds, void* codes_t,
+                  int64_t ldqt, void* scales_t, int64_t ldst, void* stream);
+/* C[M][N] = act(X W^T + bias) or X W^T + bias + residual, summed in fp32, rounded once to C's type (bf16, or fp32 when out_f32; the
+ * residual has C's type).  X: codes and scales as above -- or, when x is given, the unquantised activations x [M][K], and X / sx is
+ * scratch of the same layout that may be written.  W2 given: the gated form; W and W2 are two weights of one shape and
+ * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H [M][ldh], sh [M][ldsh] (the wi_0 / wi_1 pair of a gated feed-forward; no C, bias,
+ * residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product.                                                */
+typedef struct fdmi_fp8_desc {
+  int32_t M, N, K;
+  const void* x; int64_t ldxr; int32_t x_f32;
+  void* X; int64_t ldx; void* sx; int64_t ldsx;
+  const void* W; int64_t ldw; const void* sw; int64_t ldsw;
+  const void* W2; const void* sw2;
+  const float* bias;
+  const void* residual; int64_t ldr;
+  void* C; int64_t ldc; int32_t out_f32; int32_t act;
+  void* H; int64_t ldh; void* sh; int64_t ldsh;
+} fdmi_fp8_desc;
+int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream);
+
+/* ---------------- token-embedding lookup and its gradient (csrc/embed.hip) ----------------
+ * out[i][:] = scale * table[ids[i]][:] + pos[i mod pos_rows][:]  (table fp32 or bf16 [V][D], pos fp32 or NULL, ids int32 or int64,
+ * out bf16 or fp32 [n][D]): the text encoders' token (+ position) embedding.  An id outside [0, V) gives a row of NaN.
+ * grad[v][:] (+)= scale * sum over ids[i] == v of dy[i][:], fp32 sums in a fixed order (positions ascending in fixed chunks): two
+ * runs are bit-identical.  accumulate = 0 writes every row of grad [V][ldg], 1 adds to the rows that occur.  ws: scratch of
+ * fdmi_embed_bwd_ws_bytes(n, D) bytes, 16-byte aligned.                                                                              */
+int fdmi_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n, float scale,
+                   const float* pos, int64_t pos_rows, int64_t ldp, void* out, int out_f32, void* stream);
+int64_t fdmi_embed_bwd_ws_bytes(int64_t n, int D);
+int fdmi_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
+                   int accumulate, float* grad, int64_t ldg, void* ws, void* stream);
+
 /* ---------------- fp32 VALIDATION MODE, op level (csrc/ref32.hip) --------------------------------------------------
  * north_star asks for loss parity with the reference's CPU path to 1e-3 relative; bf16 storage cannot give that on a
  * loss that sits behind nine denoiser evaluations (and neither can the reference's own bf16-mixed run).

@@ -1,0 +1,162 @@
+"""The token-embedding lookup and its table's gradient (csrc/embed.hip) against 64-bit plain forms."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+HALF = {BF16: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+def _ops():
+    from flash_diffusion_amd import ops
+    return ops
+
+
+def _rand(*shape, seed=0, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+@pytest.mark.parametrize("tt,ot,it", [(F32, BF16, torch.int64), (F32, F32, torch.int32), (BF16, BF16, torch.int32), (BF16, F32, torch.int64)])
+@pytest.mark.parametrize("B,S,V,D", [(1, 1, 1, 1), (2, 77, 500, 768), (3, 5, 40, 7), (1, 130, 1000, 65), (4, 16, 33, 130), (2, 9, 90, 1028)])
+def test_lookup(B, S, V, D, tt, ot, it):
+    ops = _ops()
+    g = torch.Generator().manual_seed(B * S + D)
+    table, ids, pos = _rand(V, D, seed=1, dtype=tt), torch.randint(0, V, (B, S), generator=g).to(it), _rand(S + 3, D, seed=2)
+    for scale, p in ((1.0, None), (0.5, pos), (D ** 0.5, None), (-3.0, pos)):
+        got = ops.embed_fwd(table.cuda(), ids.cuda(), scale=scale, pos=None if p is None else p.cuda(), dtype=ot)
+        # (the scale travels as fp32)
+        ref = _np(table)[ids.numpy()] * float(np.float32(scale)) + (0.0 if p is None else _np(p)[None, :S])
+        assert got.shape == (B, S, D) and got.dtype == ot
+        # one fused multiply-add in fp32 and one rounding to the result's type (fp32: the first is the last)
+        e = np.abs(ref) * (HALF[ot] + (2.0 ** -24 if ot == BF16 else 0.0)) * (1 + 2.0 ** -8)
+        assert (np.abs(_np(got) - ref) <= e).all()
+
+
+def test_lookup_of_one_unscaled_row_is_a_copy_and_of_a_strided_table_too():
+    ops = _ops()
+    wide = _rand(20, 50, seed=3).cuda()
+    ids = torch.tensor([3, 0, 19, 3], device="cuda")
+    assert torch.equal(ops.embed_fwd(wide[:, 5:38], ids, dtype=F32), wide[:, 5:38][ids])
+    assert torch.equal(ops.embed_fwd(wide[::2, 1:34], ids[:2], dtype=BF16), wide[::2, 1:34][ids[:2]].to(BF16))
+    assert ops.embed_fwd(wide, torch.empty(2, 0, dtype=torch.int64, device="cuda")).shape == (2, 0, 50)
+    assert torch.equal(ops.embed_fwd(wide, torch.tensor(4, device="cuda"), dtype=F32), wide[4])
+
+
+def test_an_id_outside_the_table_reads_as_nan_and_gets_no_gradient():
+    ops = _ops()
+    table = _rand(10, 24).cuda()
+    ids = torch.tensor([[1, 10, -1], [9, 2 ** 40, 0]], device="cuda")
+    y = ops.embed_fwd(table, ids, dtype=F32)
+    bad = torch.tensor([[False, True, True], [False, True, False]], device="cuda")
+    assert bool(torch.isnan(y[bad]).all()) and torch.equal(y[~bad], table[ids[~bad]])
+    g = ops.embed_bwd(torch.ones(2, 3, 24, device="cuda"), ids, 10)
+    want = torch.zeros(10, 24, device="cuda")
+    want[[0, 1, 9]] = 1.0
+    assert torch.equal(g, want)
+
+
+def _ids_of(kind, n, V, seed):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "one":
+        return torch.full((n,), V // 2)
+    if kind == "all":
+        return torch.randperm(max(n, V), generator=g)[:n] % V
+    if kind == "runs":            # runs of 1, 2, 3, ... positions that end inside, at and behind a chunk's edge, shuffled
+        ids = torch.cat([torch.full((k,), k % V) for k in range(1, 2 + int((2 * n) ** 0.5))])[:n]
+        return torch.cat([ids, torch.zeros(n - ids.numel(), dtype=torch.long)])[torch.randperm(n, generator=g)]
+    ids = torch.randint(0, V, (n,), generator=g)          # "padded": two thirds are id 0
+    return torch.where(torch.rand(n, generator=g) < 0.67, torch.zeros_like(ids), ids)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("kind", ["one", "all", "runs", "padded"])
+@pytest.mark.parametrize("n,V,D", [(1, 1, 1), (31, 7, 3), (32, 50, 64), (33, 50, 65), (64, 300, 130), (257, 100, 257), (1232, 2000, 96), (5000, 700, 40)])
+def test_gradient(n, V, D, kind, dt):
+    ops = _ops()
+    ids = _ids_of(kind, n, V, n + V)
+    dy = _rand(n, D, seed=n, dtype=dt)
+    got = ops.embed_bwd(dy.cuda(), ids.cuda(), V, scale=0.75)
+    v = _np(dy)
+    ref, mag, cnt = np.zeros((V, D)), np.zeros((V, D)), np.zeros((V, 1))
+    np.add.at(ref, ids.numpy(), v)
+    np.add.at(mag, ids.numpy(), np.abs(v))
+    np.add.at(cnt, ids.numpy(), 1.0)
+    # count - 1 rounded additions of partial sums that never exceed mag, and the scale's product
+    assert (np.abs(_np(got) - 0.75 * ref) <= 0.75 * (cnt + 1) * 2.0 ** -24 * mag).all()
+    again = ops.embed_bwd(dy.cuda(), ids.cuda().to(torch.int32), V, scale=0.75)
+    assert torch.equal(got, again)                                     # a fixed order: the same bits
+
+
+def test_gradient_accumulates_into_strided_rows_and_leaves_the_others():
+    ops = _ops()
+    n, V, D = 200, 64, 70
+    ids = _ids_of("padded", n, V // 2, 3)
+    dy = _rand(4, n // 4, D + 6, seed=1).cuda()[..., 3:3 + D]
+    big = _rand(V, D + 5, seed=2).cuda()
+    out = big[:, 2:2 + D]
+    before = big.clone()
+    assert ops.embed_bwd(dy, ids.view(4, -1).cuda(), V, out=out) is out
+    ref, mag = np.zeros((V, D)), np.zeros((V, D))
+    np.add.at(ref, ids.numpy(), _np(dy).reshape(n, D))
+    np.add.at(mag, ids.numpy(), np.abs(_np(dy).reshape(n, D)))
+    b = _np(before)[:, 2:2 + D]
+    cnt = np.bincount(ids.numpy(), minlength=V)[:, None]
+    assert (np.abs(_np(out) - (b + ref)) <= (cnt + 2) * 2.0 ** -24 * (mag + np.abs(b))).all()
+    hit = torch.tensor(np.bincount(ids.numpy(), minlength=V) > 0, device="cuda")
+    assert torch.equal(out[~hit], before[:, 2:2 + D][~hit])
+    assert torch.equal(big[:, :2], before[:, :2]) and torch.equal(big[:, 2 + D:], before[:, 2 + D:])
+
+
+def test_gradient_of_no_tokens_is_zero():
+    ops = _ops()
+    e = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert not ops.embed_bwd(torch.empty(0, 9, device="cuda"), e, 5).any()
+    out = torch.ones(5, 9, device="cuda")
+    assert bool((ops.embed_bwd(torch.empty(0, 9, device="cuda"), e, 5, out=out) == 1).all())
+
+
+def test_a_graph_replays_lookup_and_gradient():
+    ops = _ops()
+    V, D, B, S = 90, 72, 3, 50
+    table, dy = _rand(V, D).cuda(), _rand(B, S, D, seed=1).cuda()
+    ids = _ids_of("padded", B * S, V, 1).view(B, S).cuda()
+
+    def step():
+        return ops.embed_fwd(table, ids), ops.embed_bwd(dy, ids, V)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (2, 3, 4):
+        ids.copy_(_ids_of("padded", B * S, V, seed).view(B, S))
+        dy.copy_(_rand(B, S, D, seed=seed))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+
+
+def test_refusals_on_the_gpu():
+    ops = _ops()
+    t, ids = _rand(10, 8).cuda(), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    bad = [lambda: ops.embed_fwd(t.cpu(), ids), lambda: ops.embed_fwd(t, ids.cpu()), lambda: ops.embed_fwd(t, ids.float()),
+           lambda: ops.embed_fwd(t.t(), ids), lambda: ops.embed_fwd(t.half(), ids), lambda: ops.embed_fwd(t, ids, pos=t[:2]),
+           lambda: ops.embed_fwd(t, ids, pos=t[:, :7]), lambda: ops.embed_fwd(t, ids, pos=t.bfloat16()), lambda: ops.embed_fwd(t, ids, dtype=torch.float16),
+           lambda: ops.embed_fwd(t[:0], ids), lambda: ops.embed_bwd(t, ids, 10), lambda: ops.embed_bwd(torch.zeros(2, 3, 8, device="cuda").half(), ids, 10),
+           lambda: ops.embed_bwd(torch.zeros(2, 3, 8, device="cuda"), ids, 10, out=torch.zeros(9, 8, device="cuda")),
+           lambda: ops.embed_bwd(torch.zeros(2, 3, 8, device="cuda"), ids, 10, out=torch.zeros(10, 8, dtype=BF16, device="cuda")),
+           lambda: ops.embed_bwd(torch.zeros(2, 3, 8, device="cuda"), ids, 0)]
+    for i, f in enumerate(bad):
+        with pytest.raises((ValueError, RuntimeError)):
+            f()
+            pytest.fail(f"case {i} was accepted")

@@ -1,0 +1,98 @@
+"""CPU: what the 8-bit product and embedding entry points refuse before anything is launched, and the wrappers' checks of host tensors."""
+import ctypes as C
+
+import pytest
+import torch
+
+P = 1 << 20          # an address that is aligned and never read: every call below is refused by its arguments
+
+
+def _lib():
+    from flash_diffusion_amd import _lib
+    return _lib
+
+
+def _desc(**kw):
+    d = _lib().Fp8Desc()
+    base = dict(M=4, N=64, K=130, X=P, ldx=256, sx=P, ldsx=4, W=P, ldw=256, sw=P, ldsw=4, C=P, ldc=64)
+    for k, v in {**base, **kw}.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw", [
+    dict(M=-1), dict(N=0), dict(K=0), dict(X=None), dict(X=P + 8), dict(ldx=128), dict(ldx=260), dict(sx=None), dict(sx=P + 2), dict(ldsx=2),
+    dict(ldsx=6), dict(W=None), dict(W=P + 4), dict(ldw=192), dict(sw=None), dict(ldsw=0), dict(C=None), dict(ldc=63), dict(act=2), dict(act=6),
+    dict(act=-1), dict(act=3, residual=P, ldr=64), dict(residual=P, ldr=63), dict(x=P, ldxr=129), dict(x=P, ldxr=130, ldx=384), dict(H=P),
+    dict(x=P, ldxr=130, ldsx=8), dict(ldw=1 << 22), dict(K=700, ldx=768, ldw=768, ldsx=4, ldsw=8),
+    # the gated form
+    dict(W2=P, sw2=P), dict(W2=P, sw2=P, C=None), dict(W2=P, C=None, H=P, ldh=128, sh=P, ldsh=4), dict(W2=P + 8, sw2=P, C=None, H=P, ldh=128, sh=P, ldsh=4),
+    dict(W2=P, sw2=P, C=None, H=P, ldh=64, sh=P, ldsh=4), dict(W2=P, sw2=P, C=None, H=P, ldh=128, sh=P, ldsh=0), dict(W2=P, sw2=P, C=None, bias=P, H=P, ldh=128, sh=P, ldsh=4),
+    dict(W2=P, sw2=P, C=None, act=5, H=P, ldh=128, sh=P, ldsh=4),
+])
+def test_gemm_fp8_refuses(kw):
+    L = _lib().lib()
+    d = _desc(**kw)
+    assert L.fdmi_gemm_fp8(C.byref(d), None) != 0
+    assert b"gemm_fp8" in L.fdmi_last_error()
+
+
+def test_empty_calls_are_accepted_without_a_gpu():
+    L = _lib().lib()
+    assert L.fdmi_gemm_fp8(C.byref(_desc(M=0)), None) == 0
+    assert L.fdmi_quant_fp8(None, 0, 130, None, 0.0, None, 256, None, 4, 0, 130, None) == 0
+    assert L.fdmi_embed_fwd(None, 1, 10, 8, 8, None, 1, 0, 1.0, None, 0, 0, None, 0, None) == 0
+    assert L.fdmi_embed_bwd_ws_bytes(0, 8) == 0 and L.fdmi_embed_bwd_ws_bytes(33, 8) >= 33 * 8 + 2 * 2 * 8 * 4
+
+
+@pytest.mark.parametrize("args", [
+    (None, 0, 130, None, 0.0, P, 256, P, 4, 3, 130), (P, 0, 129, None, 0.0, P, 256, P, 4, 3, 130), (P, 0, 130, None, 0.0, P, 384, P, 4, 3, 130),
+    (P, 0, 130, None, 0.0, P + 1, 256, P, 4, 3, 130), (P, 0, 130, None, 0.0, P, 256, P, 8, 3, 130), (P, 0, 130, None, 0.0, P, 256, P, 4, -3, 130),
+    (P, 0, 130, None, 0.0, P, 256, P, 4, 3, 0)])
+def test_quant_fp8_refuses(args):
+    L = _lib().lib()
+    assert L.fdmi_quant_fp8(*args, None) != 0 and b"quant_fp8" in L.fdmi_last_error()
+
+
+@pytest.mark.parametrize("args", [
+    (P, 1, 130, 0, 130, P, 256, P, 4, None, 0, None, 0), (None, 1, 130, 64, 130, P, 256, P, 4, None, 0, None, 0), (P, 1, 100, 64, 130, P, 256, P, 4, None, 0, None, 0),
+    (P, 1, 130, 64, 130, P, 130, P, 4, None, 0, None, 0), (P, 1, 130, 64, 130, P, 256, None, 4, None, 0, None, 0), (P, 1, 130, 64, 130, P, 256, P, 4, P, 64, P, 4),
+    (P, 1, 130, 64, 130, P, 256, P, 4, P, 128, None, 4)])
+def test_pack_fp8_refuses(args):
+    L = _lib().lib()
+    assert L.fdmi_pack_fp8(*args, None) != 0 and b"pack_fp8" in L.fdmi_last_error()
+
+
+def test_embed_refuses():
+    L = _lib().lib()
+    for a in ((P, 1, 0, 8, 8, P, 1, 3, 1.0, None, 0, 0, P, 0), (P, 1, 10, 0, 8, P, 1, 3, 1.0, None, 0, 0, P, 0), (P, 1, 10, 8, 7, P, 1, 3, 1.0, None, 0, 0, P, 0),
+              (P, 1, 10, 8, 8, None, 1, 3, 1.0, None, 0, 0, P, 0), (P, 1, 10, 8, 8, P, 1, 3, 1.0, P, 0, 8, P, 0), (P, 1, 10, 8, 8, P, 1, 3, 1.0, P, 3, 7, P, 0),
+              (P, 1, 10, 8, 8, P, 1, -1, 1.0, None, 0, 0, P, 0), (P, 1, 10, 8, 8, P, 1, 3, 1.0, None, 0, 0, None, 0), (P, 1, 1 << 31, 8, 8, P, 1, 3, 1.0, None, 0, 0, P, 0)):
+        assert L.fdmi_embed_fwd(*a, None) != 0 and b"embed_fwd" in L.fdmi_last_error()
+    for a in ((P, 1, 8, P, 1, 3, 0, 8, 1.0, 0, P, 8, P), (P, 1, 7, P, 1, 3, 10, 8, 1.0, 0, P, 8, P), (P, 1, 8, P, 1, 3, 10, 8, 1.0, 0, P, 7, P), (P, 1, 8, P, 1, 3, 10, 8, 1.0, 0, None, 8, P),
+              (P, 1, 8, P, 1, 3, 10, 8, 1.0, 0, P, 8, None), (P, 1, 8, P, 1, 3, 10, 8, 1.0, 0, P, 8, P + 4), (P, 1, 8, P, 1, 1 << 31, 10, 8, 1.0, 0, P, 8, P)):
+        assert L.fdmi_embed_bwd(*a, None) != 0 and b"embed_bwd" in L.fdmi_last_error()
+
+
+def test_wrappers_refuse_host_tensors():
+    from flash_diffusion_amd import ops
+    x = torch.zeros(4, 130)
+    for f in (lambda: ops.quant_fp8(x), lambda: ops.rmsnorm_fp8(x, torch.ones(130), 1e-6), lambda: ops.pack_weight_fp8(x),
+              lambda: ops.embed_fwd(x, torch.zeros(3, dtype=torch.int64)), lambda: ops.embed_bwd(x, torch.zeros(4, dtype=torch.int64), 9)):
+        with pytest.raises(ValueError, match="current GPU"):
+            f()
+
+
+def test_the_reference_quantiser_agrees_with_torchs_cast():
+    """the 64-bit form the GPU tests compare with, against torch's own e4m3 rounding of the scaled values (CPU)"""
+    import numpy as np
+    from tests import fp8_ref as R
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(9, 700, generator=g) * torch.exp(3 * torch.randn(700, generator=g))
+    got, exps = R.quantise(x.numpy())
+    s = torch.from_numpy(2.0 ** np.repeat(exps, 128, 1)[:, :700].astype(np.float64))
+    want = (x.double() / s).float().to(torch.float8_e4m3fn).double() * s
+    assert np.array_equal(got, want.numpy())
+    m = np.abs(np.pad(x.numpy(), ((0, 0), (0, 68))).reshape(9, 6, 128)).max(2)
+    sc = 2.0 ** exps.astype(np.float64)
+    assert (m <= 448 * sc).all() and (m > 224 * sc).all()
