@@ -41,9 +41,9 @@ class WgradProblem(C.Structure):
 
 class Fp8Desc(C.Structure):
     """fdmi_fp8_desc (include/fdmi.h)"""
-    _fields_ = [("M", i32), ("N", i32), ("K", i32), ("x", vp), ("ldxr", i64), ("x_f32", i32), ("X", vp), ("ldx", i64), ("sx", vp),
-                ("ldsx", i64), ("W", vp), ("ldw", i64), ("sw", vp), ("ldsw", i64), ("W2", vp), ("sw2", vp), ("bias", vp), ("residual", vp),
-                ("ldr", i64), ("C", vp), ("ldc", i64), ("out_f32", i32), ("act", i32), ("H", vp), ("ldh", i64), ("sh", vp), ("ldsh", i64)]
+    _fields_ = [("M", i32), ("N", i32), ("K", i32), ("x", vp), ("ldxr", i64), ("x_f32", i32), ("X", vp), ("sx", vp), ("W", vp), ("sw", vp),
+                ("W2", vp), ("sw2", vp), ("bias", vp), ("residual", vp), ("ldr", i64), ("C", vp), ("ldc", i64), ("out_f32", i32),
+                ("act", i32), ("H", vp), ("sh", vp)]
 
 
 class UNetCfg(C.Structure):
@@ -153,8 +153,8 @@ _SIGS = {
     "fdmi_distill_grad": (i32, [vp, vp, i64, i32, f32, vp, vp]),
     "fdmi_dmd_loss": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i64, vp]),
     # 8-bit block-scaled products (csrc/fp8.hip) and the embedding lookup (csrc/embed.hip)
-    "fdmi_quant_fp8": (i32, [vp, i32, i64, vp, f32, vp, i64, vp, i64, i64, i32, vp]),
-    "fdmi_pack_fp8": (i32, [vp, i32, i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp]),
+    "fdmi_quant_fp8": (i32, [vp, i32, i64, vp, f32, vp, vp, i64, i32, vp]),
+    "fdmi_pack_fp8": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp]),
     "fdmi_gemm_fp8": (i32, [C.POINTER(Fp8Desc), vp]),
     "fdmi_embed_fwd": (i32, [vp, i32, i64, i32, i64, vp, i32, i64, f32, vp, i64, i64, vp, i32, vp]),
     "fdmi_embed_bwd_ws_bytes": (i64, [i64, i32]),

@@ -449,50 +449,42 @@ int fdmi_pad_cols_f32(const float* src, int cols, float* dst, int cols_pad, int6
 
 // ---- 8-bit products (fp8.hip) and the embedding lookup (embed.hip) ----
 namespace {
-bool fp8_codes_ok(const void* p, int64_t ld, int64_t cols) {
-  return p && ((uintptr_t)p & 15) == 0 && ld % 128 == 0 && ld >= cols && ld < (1 << 22);
+// codes and scales of an 8-bit operand, the contraction short enough for 32-bit offsets into a tile of 256 rows
+bool fp8_ok(const void* codes, const void* scales, int64_t K) {
+  return codes && ((uintptr_t)codes & 15) == 0 && scales && ((uintptr_t)scales & 3) == 0 && K < (1 << 22);
 }
-bool fp8_scales_ok(const void* p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p & 3) == 0 && ld % 4 == 0 && ld * 128 >= cols; }
 }  // namespace
 
-int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, void* codes, int64_t ldq, void* scales, int64_t lds,
-                   int64_t M, int K, void* stream) {
+int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, void* codes, void* scales, int64_t M, int K,
+                   void* stream) {
   FDMI_CHECK(M >= 0 && M < (1ll << 31) && K >= 1, "quant_fp8: need M >= 0 and K >= 1");
   if (M == 0) return 0;
   FDMI_CHECK(x && ldx >= K, "quant_fp8: x rows shorter than K");
-  FDMI_CHECK(fp8_codes_ok(codes, ldq, K) && ldq == (K + 127) / 128 * 128, "quant_fp8: code rows are K padded to 128, 16-byte aligned");
-  FDMI_CHECK(fp8_scales_ok(scales, lds, K) && lds == ((K + 127) / 128 + 3) / 4 * 4, "quant_fp8: scale rows are ceil(K / 128) padded to 4 bytes");
-  return launch_quant_fp8(x, x_f32, ldx, norm, eps, (uint8_t*)codes, ldq, (uint8_t*)scales, lds, M, K, (hipStream_t)stream);
+  FDMI_CHECK(fp8_ok(codes, scales, K), "quant_fp8: codes are 16-byte, scales 4-byte aligned, K < 4M");
+  return launch_quant_fp8(x, x_f32, ldx, norm, eps, (uint8_t*)codes, (uint8_t*)scales, M, K, (hipStream_t)stream);
 }
-int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, int64_t ldq, void* scales, int64_t lds, void* codes_t,
-                  int64_t ldqt, void* scales_t, int64_t ldst, void* stream) {
+int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t,
+                  void* stream) {
   FDMI_CHECK(N >= 1 && K >= 1 && w && ldw >= K, "pack_fp8: need a weight [N][K]");
-  FDMI_CHECK((int64_t)N < (1 << 22) && (int64_t)K < (1 << 22), "pack_fp8: weights up to 4M rows and columns");
-  FDMI_CHECK(fp8_codes_ok(codes, ldq, ((int64_t)K + 127) / 128 * 128) && fp8_scales_ok(scales, lds, K), "pack_fp8: codes / scales layout");
-  if (codes_t)
-    FDMI_CHECK(fp8_codes_ok(codes_t, ldqt, ((int64_t)N + 127) / 128 * 128) && fp8_scales_ok(scales_t, ldst, N), "pack_fp8: transposed layout");
-  return launch_pack_fp8(w, w_f32, ldw, N, K, (uint8_t*)codes, ldq, (uint8_t*)scales, lds, (uint8_t*)codes_t, ldqt, (uint8_t*)scales_t, ldst,
-                         (hipStream_t)stream);
+  FDMI_CHECK(fp8_ok(codes, scales, K) && (!codes_t || fp8_ok(codes_t, scales_t, N)) && N < (1 << 22),
+             "pack_fp8: codes are 16-byte, scales 4-byte aligned, N and K < 4M");
+  return launch_pack_fp8(w, w_f32, ldw, N, K, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)codes_t, (uint8_t*)scales_t, (hipStream_t)stream);
 }
 int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
   FDMI_CHECK(d && d->M >= 0 && d->N >= 1 && d->K >= 1, "gemm_fp8: need M >= 0, N >= 1, K >= 1");
   if (d->M == 0) return 0;
-  const int64_t Kp = ((int64_t)d->K + 127) / 128 * 128, ls = (Kp / 128 + 3) / 4 * 4;
-  FDMI_CHECK(fp8_codes_ok(d->X, d->ldx, Kp) && fp8_scales_ok(d->sx, d->ldsx, d->K), "gemm_fp8: layout of X's codes / scales");
-  FDMI_CHECK(fp8_codes_ok(d->W, d->ldw, Kp) && fp8_scales_ok(d->sw, d->ldsw, d->K), "gemm_fp8: layout of W's codes / scales");
-  FDMI_CHECK(d->ldsx >= ls && d->ldsw >= ls, "gemm_fp8: scale rows are padded to four bytes");
-  FDMI_CHECK(!d->x || (d->ldxr >= d->K && d->ldx == Kp && d->ldsx == ls), "gemm_fp8: unquantised rows need scratch codes [M][K padded to 128]");
+  FDMI_CHECK(fp8_ok(d->X, d->sx, d->K) && fp8_ok(d->W, d->sw, d->K), "gemm_fp8: codes are 16-byte, scales 4-byte aligned, K < 4M");
+  FDMI_CHECK(!d->x || d->ldxr >= d->K, "gemm_fp8: x rows shorter than K");
   Fp8GemmArgs a;
-  a.X = (const uint8_t*)d->X; a.ldx = d->ldx; a.sx = (const uint8_t*)d->sx; a.ldsx = d->ldsx;
-  a.W = (const uint8_t*)d->W; a.ldw = d->ldw; a.sw = (const uint8_t*)d->sw; a.ldsw = d->ldsw;
-  a.M = d->M; a.N = d->N; a.Kb = (int)(Kp / 128);
+  a.X = (const uint8_t*)d->X; a.sx = (const uint8_t*)d->sx;
+  a.W = (const uint8_t*)d->W; a.sw = (const uint8_t*)d->sw;
+  a.M = d->M; a.N = d->N; a.Kb = cdiv(d->K, 128);
   if (d->W2) {
-    const int64_t Np = ((int64_t)d->N + 127) / 128 * 128;
-    FDMI_CHECK(((uintptr_t)d->W2 & 15) == 0 && d->sw2 && ((uintptr_t)d->sw2 & 3) == 0, "gemm_fp8: W2 is a second weight of W's layout");
+    FDMI_CHECK(fp8_ok(d->W2, d->sw2, d->K), "gemm_fp8: W2 is a second weight of W's shape");
     FDMI_CHECK(!d->C && !d->bias && !d->residual && d->act == 0, "gemm_fp8: the gated form takes no C, bias, residual or act");
-    FDMI_CHECK(fp8_codes_ok(d->H, d->ldh, Np) && fp8_scales_ok(d->sh, d->ldsh, d->N), "gemm_fp8: layout of H's codes / scales");
+    FDMI_CHECK(fp8_ok(d->H, d->sh, d->N), "gemm_fp8: the gated form writes codes H and scales sh");
     a.W2 = (const uint8_t*)d->W2; a.sw2 = (const uint8_t*)d->sw2;
-    a.H = (uint8_t*)d->H; a.ldh = d->ldh; a.sh = (uint8_t*)d->sh; a.ldsh = d->ldsh;
+    a.H = (uint8_t*)d->H; a.sh = (uint8_t*)d->sh;
   } else {
     FDMI_CHECK(d->C && d->ldc >= d->N, "gemm_fp8: C rows shorter than N");
     FDMI_CHECK(!d->H && !d->sh, "gemm_fp8: H belongs to the gated form");
@@ -503,8 +495,7 @@ int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
     a.bias = d->bias; a.residual = d->residual; a.ldr = d->ldr; a.C = d->C; a.ldc = d->ldc; a.out_f32 = d->out_f32; a.act = d->act;
   }
   if (d->x) {
-    const int rc = launch_quant_fp8(d->x, d->x_f32, d->ldxr, nullptr, 0.f, (uint8_t*)d->X, d->ldx, (uint8_t*)d->sx, d->ldsx, d->M, d->K,
-                                    (hipStream_t)stream);
+    const int rc = launch_quant_fp8(d->x, d->x_f32, d->ldxr, nullptr, 0.f, (uint8_t*)d->X, (uint8_t*)d->sx, d->M, d->K, (hipStream_t)stream);
     if (rc) return rc;
   }
   return launch_gemm_fp8(a, (hipStream_t)stream);

@@ -2,29 +2,23 @@
 #pragma once
 #include "common.h"
 
-// One product  C[M][N] = act(X W^T + bias + residual)  of e4m3 codes.  X codes [M][ldx] with one scale byte per row and 128 columns,
-// W codes [N][ldw] with one per 128 rows and 128 columns; both padded with zero codes to whole blocks (Kb of them) along the contraction,
-// scale rows padded to a multiple of four bytes.  gated: W2 is a second weight of the same form and the result
-// gelu_tanh(X W^T) * (X W2^T) leaves as codes H [M][ldh] with scales sh instead of C.
+// One product  C[M][N] = act(X W^T + bias + residual)  of e4m3 codes in tiles (fp8.hip); Kb blocks of 128 along the contraction.  gated:
+// W2 is a second weight of the same form and the result gelu_tanh(X W^T) * (X W2^T) leaves as codes H with scales sh instead of C.
 struct Fp8GemmArgs {
-  const uint8_t* X = nullptr; int64_t ldx = 0;
-  const uint8_t* sx = nullptr; int64_t ldsx = 0;
-  const uint8_t* W = nullptr; int64_t ldw = 0;
-  const uint8_t* sw = nullptr; int64_t ldsw = 0;
-  const uint8_t* W2 = nullptr; const uint8_t* sw2 = nullptr;   // (leading dimensions as W's)
+  const uint8_t* X = nullptr; const uint8_t* sx = nullptr;
+  const uint8_t* W = nullptr; const uint8_t* sw = nullptr;
+  const uint8_t* W2 = nullptr; const uint8_t* sw2 = nullptr;
   int M = 0, N = 0, Kb = 0;
   const float* bias = nullptr;
   const void* residual = nullptr; int64_t ldr = 0;             // of C's type
   void* C = nullptr; int64_t ldc = 0; int out_f32 = 0;
   int act = 0;
-  uint8_t* H = nullptr; int64_t ldh = 0;
-  uint8_t* sh = nullptr; int64_t ldsh = 0;
+  uint8_t* H = nullptr; uint8_t* sh = nullptr;
 };
 int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st);
-int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, uint8_t* q, int64_t ldq, uint8_t* s, int64_t lds,
-                     int64_t M, int K, hipStream_t st);
-int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t* q, int64_t ldq, uint8_t* s, int64_t lds, uint8_t* qt,
-                    int64_t ldqt, uint8_t* st, int64_t ldst, hipStream_t stream);
+int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, uint8_t* q, uint8_t* s, int64_t M, int K,
+                     hipStream_t st);
+int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st, hipStream_t stream);
 
 // ---- embed.hip ----
 int launch_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n, float scale,

@@ -415,11 +415,17 @@ def attn_bwd(q, k, v, o, do, lse, H, scale, out=None):
 
 # ---- 8-bit products with a scale for each block of 128 (csrc/fp8.hip) -----------------------------------------------------------
 F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _stream():
+    """the current device's current stream, without the Stream object that stream_ptr() makes on the way"""
+    return _raw_stream(_current())
 
 
 def _here(t, what):
     """an operand of the 8-bit / embedding entry points: on the current device (their launches go to its current stream)"""
-    if not (t.is_cuda and t.get_device() == torch.cuda.current_device()):
+    if not t.is_cuda or t.get_device() != _current():
         raise ValueError(f"{what} is on {t.device}: it has to be on the current GPU")
     return t
 
@@ -429,51 +435,76 @@ def _rows(t, what, dtypes=(BF16, F32)):
     _here(t, what)
     if t.dim() != 2 or t.dtype not in dtypes:
         raise ValueError(f"{what}: need a 2-D tensor of {dtypes}, got {tuple(t.shape)} {t.dtype}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    M, K = t.shape
+    ld, inner = t.stride()
+    if inner != 1 and K > 1:
         raise ValueError(f"{what}: the last dimension has to be contiguous")
-    if t.shape[0] > 1:
-        if t.stride(0) < t.shape[1]:
-            raise ValueError(f"{what}: rows overlap (stride {t.stride(0)} < {t.shape[1]})")
-        return t.stride(0)
-    return t.shape[1]
+    if M <= 1:
+        return K
+    if ld < K:
+        raise ValueError(f"{what}: rows overlap (stride {ld} < {K})")
+    return ld
+
+
+def _vector(t, n, what):
+    _here(t, what)
+    if t.dtype != F32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what}: need a contiguous fp32 [{n}], got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
 
 
 def _pad(n, to):
     return -(-n // to) * to
 
 
+def _untile(codes, rows, K):
+    """codes in their tiles (include/fdmi.h) -> [rows, K] e4m3"""
+    t = codes.view(-1, 2 * _pad(K, 128) // 128, 4, 16, 16).permute(0, 3, 1, 2, 4)
+    return t.reshape(-1, _pad(K, 128))[:rows, :K].view(F8)
+
+
 class Fp8Rows:
-    """Rows of activations in 8 bits: codes [M, K padded to 128] e4m3 (zeros behind K), scales [M, K / 128 padded to 4] e8m0, one for
-    each 128 columns.  The value of a code is code * scale; .values() gives them as [M, K]."""
+    """Rows of activations [M, K] in 8 bits: e4m3 codes in tiles, a power-of-two scale for each row and 128 columns (include/fdmi.h has the
+    layout).  .values() reads them back."""
+    __slots__ = ("M", "K", "codes", "scales")
 
     def __init__(self, M, K, device):
-        self.M, self.K, self.Kp, self.Ks = M, K, _pad(K, 128), _pad(_pad(K, 128) // 128, 4)
-        self.codes = torch.empty(M, self.Kp, dtype=F8, device=device)
-        self.scales = torch.empty(M, self.Ks, dtype=E8, device=device)
+        self.M, self.K = M, K
+        Mp, Kb = _pad(M, 16), _pad(K, 128) // 128
+        b = torch.empty(Mp * Kb * 129, dtype=torch.uint8, device=device)
+        self.codes, self.scales = b[:Mp * Kb * 128], b[Mp * Kb * 128:]
+
+    def parts(self):
+        """(codes [M, K] e4m3, scales [M, ceil(K / 128)] e8m0): a value is its code times its block's scale"""
+        Kb = _pad(self.K, 128) // 128
+        return _untile(self.codes, self.M, self.K), self.scales.view(Kb, _pad(self.M, 16)).t()[:self.M].contiguous().view(E8)
 
     def values(self, dtype=F32):
         """read back (a test / debugging aid in torch operations; e4m3 times a power of two is exact in bf16 and fp32)"""
-        c = self.codes.float().view(self.M, self.Kp // 128, 128) * self.scales[:, :self.Kp // 128].float()[..., None]
-        return c.view(self.M, self.Kp)[:, :self.K].to(dtype)
+        c, s = self.parts()
+        return (c.float() * s.float().repeat_interleave(128, 1)[:, :self.K]).to(dtype)
 
 
 class Fp8Weight:
-    """A frozen weight [N, K] in 8 bits: codes [N, K padded to 128], scales [ceil(N / 128), K / 128 padded to 4], one for each 128 x 128
-    block; codes_t / scales_t (or None): the transpose, which gemm_fp8_dgrad contracts with."""
+    """A frozen weight [N, K] in 8 bits: e4m3 codes in tiles, a power-of-two scale for each 128 x 128 block; codes_t / scales_t (or None): its
+    transpose, which gemm_fp8_dgrad contracts with."""
+    __slots__ = ("N", "K", "codes", "scales", "codes_t", "scales_t")
 
     def __init__(self, N, K, device, transposed):
-        self.N, self.K, self.Kp, self.Np = N, K, _pad(K, 128), _pad(N, 128)
-        # (scale rows are padded to 4: the padding is never read as a scale, but initialised memory is easier to look at)
-        self.codes = torch.empty(N, self.Kp, dtype=F8, device=device)
-        self.scales = torch.zeros(self.Np // 128, _pad(self.Kp // 128, 4), dtype=torch.uint8, device=device).view(E8)
-        self.codes_t = self.scales_t = None
-        if transposed:
-            self.codes_t = torch.empty(K, self.Np, dtype=F8, device=device)
-            self.scales_t = torch.zeros(self.Kp // 128, _pad(self.Np // 128, 4), dtype=torch.uint8, device=device).view(E8)
+        self.N, self.K = N, K
+        new = lambda n, k: (torch.empty(_pad(n, 16) * _pad(k, 128), dtype=torch.uint8, device=device),
+                            torch.empty(_pad(k, 128) // 128 * (_pad(n, 128) // 32), dtype=torch.uint8, device=device))
+        self.codes, self.scales = new(N, K)
+        self.codes_t, self.scales_t = new(K, N) if transposed else (None, None)
+
+    def parts(self, transposed=False):
+        """(codes [N, K] e4m3, scales [ceil(N / 128), ceil(K / 128)] e8m0), or those of the transpose"""
+        n, k, c, s = (self.K, self.N, self.codes_t, self.scales_t) if transposed else (self.N, self.K, self.codes, self.scales)
+        return _untile(c, n, k), s.view(_pad(k, 128) // 128, -1)[:, ::4].t().contiguous().view(E8)
 
     def values(self, dtype=F32):
-        s = self.scales[:, :self.Kp // 128].float().repeat_interleave(128, 0)[:self.N].repeat_interleave(128, 1)
-        return (self.codes.float() * s)[:, :self.K].to(dtype)
+        c, s = self.parts()
+        return (c.float() * s.float().repeat_interleave(128, 0)[:self.N].repeat_interleave(128, 1)[:, :self.K]).to(dtype)
 
 
 def pack_weight_fp8(w, transposed=False):
@@ -482,8 +513,8 @@ def pack_weight_fp8(w, transposed=False):
     if w.shape[0] < 1 or w.shape[1] < 1:
         raise ValueError(f"weight is empty: {tuple(w.shape)}")
     o = Fp8Weight(w.shape[0], w.shape[1], w.device, transposed)
-    check(lib().fdmi_pack_fp8(ptr(w), int(w.dtype == F32), ld, o.N, o.K, ptr(o.codes), o.Kp, ptr(o.scales), o.scales.stride(0),
-                              ptr(o.codes_t), o.Np, ptr(o.scales_t), 0 if o.scales_t is None else o.scales_t.stride(0), stream_ptr()))
+    check(lib().fdmi_pack_fp8(ptr(w), int(w.dtype == F32), ld, o.N, o.K, ptr(o.codes), ptr(o.scales), ptr(o.codes_t), ptr(o.scales_t),
+                              _stream()))
     return o
 
 
@@ -495,63 +526,58 @@ def quant_fp8(x):
 def rmsnorm_fp8(x, w, eps):
     """x * rsqrt(mean(x^2) + eps) * w (T5LayerNorm, computed in fp32), quantised -> Fp8Rows; w [K] f32 (None: x itself)"""
     ld = _rows(x, "x")
-    if x.shape[1] < 1:
+    M, K = x.shape
+    if K < 1:
         raise ValueError(f"x has no columns: {tuple(x.shape)}")
-    if w is not None:
-        _here(w, "w")
-        if w.dtype != F32 or tuple(w.shape) != (x.shape[1],) or not w.is_contiguous():
-            raise ValueError(f"w: need a contiguous fp32 [{x.shape[1]}], got {tuple(w.shape)} {w.dtype}")
-    o = Fp8Rows(x.shape[0], x.shape[1], x.device)
-    check(lib().fdmi_quant_fp8(ptr(x), int(x.dtype == F32), ld, ptr(w), eps, ptr(o.codes), o.Kp, ptr(o.scales), o.Ks, o.M, o.K,
-                               stream_ptr()))
+    o = Fp8Rows(M, K, x.device)
+    check(lib().fdmi_quant_fp8(x.data_ptr(), x.dtype == F32, ld, None if w is None else _vector(w, K, "w"), eps, o.codes.data_ptr(),
+                               o.scales.data_ptr(), M, K, _stream()))
     return o
 
 
-def _fp8_operands(d, A, K, what):
-    """fills the activation side of a descriptor from Fp8Rows or from [M, K] bf16 / f32 rows (quantised by the call itself); returns
-    (M, device, what has to stay alive until the launch)"""
+def _fp8_rows_of(d, A, K, what):
+    """fills the activation side of a descriptor from Fp8Rows or from [M, K] bf16 / f32 rows (quantised by the call itself); returns what has
+    to stay alive until the launch"""
     if isinstance(A, Fp8Rows):
         if A.K != K:
             raise ValueError(f"{what} has {A.K} columns, the weight contracts over {K}")
-        _here(A.codes, what)
-        d.M, d.X, d.ldx, d.sx, d.ldsx = A.M, A.codes.data_ptr(), A.Kp, A.scales.data_ptr(), A.Ks
-        return A.M, A.codes.device, A
-    ld = _rows(A, what)
-    M = A.shape[0]
-    if A.shape[1] != K:
-        raise ValueError(f"{what} has {A.shape[1]} columns, the weight contracts over {K}")
-    Kp = _pad(K, 128)
-    Ks = _pad(Kp // 128, 4)
-    scratch = torch.empty(M * (Kp + Ks) + 1, dtype=torch.uint8, device=A.device)
-    d.M, d.x, d.ldxr, d.x_f32 = M, A.data_ptr(), ld, int(A.dtype == F32)
-    d.X, d.ldx, d.sx, d.ldsx = scratch.data_ptr(), Kp, scratch.data_ptr() + M * Kp, Ks
-    return M, A.device, scratch
+        d.M, d.X, d.sx = A.M, _here(A.codes, what).data_ptr(), A.scales.data_ptr()
+        return A.codes
+    d.ldxr = _rows(A, what)
+    M, cols = A.shape
+    if cols != K:
+        raise ValueError(f"{what} has {cols} columns, the weight contracts over {K}")
+    n = _pad(M, 16) * (_pad(K, 128) // 128)
+    scratch = torch.empty(n * 129, dtype=torch.uint8, device=A.device)
+    p = scratch.data_ptr()
+    d.M, d.x, d.x_f32, d.X, d.sx = M, A.data_ptr(), A.dtype == F32, p, p + n * 128
+    return scratch
 
 
 def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what):
     d = Fp8Desc()
-    d.N, d.K = N, K
-    M, dev, keep = _fp8_operands(d, A, K, what)
+    keep = _fp8_rows_of(d, A, K, what)
+    M = d.M
     if out is None:
-        out = torch.empty(M, N, dtype=F32 if out_f32 else BF16, device=dev)
-    elif tuple(out.shape) != (M, N):
-        raise ValueError(f"out: need [{M}, {N}], got {tuple(out.shape)}")
-    d.C, d.ldc, d.out_f32, d.act = out.data_ptr(), _rows(out, "out"), int(out.dtype == F32), act
-    d.W, d.ldw, d.sw, d.ldsw = codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0)
-    _here(codes, "weight")
+        out = torch.empty((M, N), dtype=F32 if out_f32 else BF16, device=keep.device)
+        d.ldc = N
+    else:
+        d.ldc = _rows(out, "out")
+        if tuple(out.shape) != (M, N):
+            raise ValueError(f"out: need [{M}, {N}], got {tuple(out.shape)}")
+    d.N, d.K, d.C, d.out_f32, d.act = N, K, out.data_ptr(), out.dtype == F32, act
+    d.W, d.sw = _here(codes, "weight").data_ptr(), scales.data_ptr()
     if bias is not None:
-        _here(bias, "bias")
-        if bias.dtype != F32 or tuple(bias.shape) != (N,) or not bias.is_contiguous():
-            raise ValueError(f"bias: need a contiguous fp32 [{N}], got {tuple(bias.shape)} {bias.dtype}")
-        d.bias = bias.data_ptr()
+        d.bias = _vector(bias, N, "bias")
     if residual is not None:
         if act != ACT_NONE:
             raise ValueError("an activation and a residual exclude each other")
+        d.ldr = _rows(residual, "residual", (out.dtype,))
         if tuple(residual.shape) != (M, N):
             raise ValueError(f"residual: need [{M}, {N}], got {tuple(residual.shape)}")
-        d.residual, d.ldr = residual.data_ptr(), _rows(residual, "residual", (out.dtype,))
+        d.residual = residual.data_ptr()
     if M:
-        check(lib().fdmi_gemm_fp8(C.byref(d), stream_ptr()))
+        check(lib().fdmi_gemm_fp8(C.byref(d), _stream()))
     return out
 
 
@@ -570,29 +596,27 @@ def gemm_fp8_dgrad(dY, W, *, residual=None, out=None, out_f32=False):
 
 def gated_fp8(A, W, W2):
     """gelu_tanh(A W^T) * (A W2^T), quantised: the gated feed-forward's first half (T5: wi_0, wi_1) -> Fp8Rows [M, N].  The product is
-    formed in fp32 and never leaves the kernel in any other form than its codes."""
+    formed in fp32 and leaves the kernels in no other form than its codes."""
     if (W.N, W.K) != (W2.N, W2.K):
         raise ValueError(f"the two weights differ in shape: {(W.N, W.K)} and {(W2.N, W2.K)}")
     d = Fp8Desc()
+    keep = _fp8_rows_of(d, A, W.K, "A")
+    o = Fp8Rows(d.M, W.N, keep.device)
     d.N, d.K = W.N, W.K
-    M, dev, keep = _fp8_operands(d, A, W.K, "A")
-    _here(W.codes, "weight")
-    _here(W2.codes, "second weight")
-    o = Fp8Rows(M, W.N, dev)
-    d.W, d.ldw, d.sw, d.ldsw = W.codes.data_ptr(), W.Kp, W.scales.data_ptr(), W.scales.stride(0)
-    d.W2, d.sw2 = W2.codes.data_ptr(), W2.scales.data_ptr()
-    d.H, d.ldh, d.sh, d.ldsh = o.codes.data_ptr(), o.Kp, o.scales.data_ptr(), o.Ks
-    if M:
-        check(lib().fdmi_gemm_fp8(C.byref(d), stream_ptr()))
+    d.W, d.sw = _here(W.codes, "weight").data_ptr(), W.scales.data_ptr()
+    d.W2, d.sw2 = _here(W2.codes, "second weight").data_ptr(), W2.scales.data_ptr()
+    d.H, d.sh = o.codes.data_ptr(), o.scales.data_ptr()
+    if d.M:
+        check(lib().fdmi_gemm_fp8(C.byref(d), _stream()))
     return o
 
 
 # ---- token embedding (csrc/embed.hip) ------------------------------------------------------------------------------------------
 def _ids(ids):
-    _here(ids, "ids")
     if ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"ids: need int32 or int64, got {ids.dtype}")
-    return ids.contiguous()
+    _here(ids, "ids")
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16):
@@ -603,17 +627,17 @@ def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16):
     V, D = table.shape
     if V < 1 or D < 1 or dtype not in (BF16, F32):
         raise ValueError(f"table {tuple(table.shape)} -> {dtype}: need rows, columns, and bf16 or fp32 out")
-    S = ids.shape[-1] if ids.dim() else 1
-    ldp = 0
+    shape = ids.shape
+    S, ldp, p = (shape[-1] if shape else 1), 0, None
     if pos is not None:
-        ldp = _rows(pos, "pos", (F32,))
+        ldp, p = _rows(pos, "pos", (F32,)), pos.data_ptr()
         if pos.shape[0] < S or pos.shape[1] != D:
             raise ValueError(f"pos: need at least [{S}, {D}], got {tuple(pos.shape)}")
-    out = torch.empty(*ids.shape, D, dtype=dtype, device=table.device)
+    out = torch.empty((*shape, D), dtype=dtype, device=table.device)
     n = ids.numel()
     if n:
-        check(lib().fdmi_embed_fwd(ptr(table), int(table.dtype == F32), V, D, ld, ptr(ids), int(ids.dtype == torch.int64), n, scale,
-                                   ptr(pos), S, ldp, ptr(out), int(dtype == F32), stream_ptr()))
+        check(lib().fdmi_embed_fwd(table.data_ptr(), table.dtype == F32, V, D, ld, ids.data_ptr(), ids.dtype == torch.int64, n, scale, p, S,
+                                   ldp, out.data_ptr(), dtype == F32, _stream()))
     return out
 
 
@@ -622,7 +646,7 @@ def embed_bwd(dy, ids, V, scale=1.0, out=None):
     accumulated into (+=) instead of a new gradient.  Sums run in a fixed order (bit-reproducible); ids outside the table are dropped."""
     ids = _ids(ids)
     D = dy.shape[-1]
-    if tuple(dy.shape[:-1]) != tuple(ids.shape) or D < 1 or V < 1:
+    if dy.shape[:-1] != ids.shape or D < 1 or V < 1:
         raise ValueError(f"dy {tuple(dy.shape)} does not match ids {tuple(ids.shape)} (V = {V})")
     n = ids.numel()
     rows = dy.reshape(n, D)
@@ -631,12 +655,13 @@ def embed_bwd(dy, ids, V, scale=1.0, out=None):
     if acc:
         if tuple(out.shape) != (V, D):
             raise ValueError(f"out: need [{V}, {D}], got {tuple(out.shape)}")
+        ldg = _rows(out, "out", (F32,))
     else:
-        out = torch.empty(V, D, dtype=F32, device=dy.device)
-    ldg = _rows(out, "out", (F32,))
-    ws = torch.empty(lib().fdmi_embed_bwd_ws_bytes(n, D), dtype=torch.uint8, device=dy.device)
-    check(lib().fdmi_embed_bwd(ptr(rows), int(dy.dtype == F32), ld, ptr(ids), int(ids.dtype == torch.int64), n, V, D, scale, int(acc),
-                               ptr(out), ldg, ptr(ws), stream_ptr()))
+        out, ldg = torch.empty((V, D), dtype=F32, device=dy.device), D
+    L = lib()
+    ws = torch.empty(L.fdmi_embed_bwd_ws_bytes(n, D), dtype=torch.uint8, device=dy.device)
+    check(L.fdmi_embed_bwd(rows.data_ptr(), dy.dtype == F32, ld, ids.data_ptr(), ids.dtype == torch.int64, n, V, D, scale, acc,
+                           out.data_ptr(), ldg, ws.data_ptr(), _stream()))
     return out
 
 

@@ -209,34 +209,34 @@ int fdmi_dmd_loss(const float* s, const float* noisy, const float* real, const f
 /* ---------------- 8-bit matrix products with a scale for each block of 128 (csrc/fp8.hip) ----------------
  * The frozen text encoders' linears (T5-XXL behind embedders/t5/t5_embedder_model.py:11-104) in 8 bits: codes are e4m3, a scale is
  * a power of two held as its biased exponent in one byte (e8m0), 2^e the smallest power with amax <= 448 2^e over the block.  A row of
- * activations has one scale per 128 columns, a weight [N][K] one per 128 x 128 block.  Code rows are padded with zeros to a multiple
- * of 128 columns (leading dimension: a multiple of 128), scale rows to a multiple of four bytes; both start 16- / 4-byte aligned.
- * An infinity or NaN becomes the NaN code and does not enter its block's scale.
+ * activations has one scale per 128 columns, a weight [N][K] one per 128 x 128 block.  An infinity or NaN becomes the NaN code and does
+ * not enter its block's scale.  Kb = ceil(K / 128), R16 = rows padded to 16:
+ *   codes   R16 * Kb * 128 bytes, 16-byte aligned: tiles [R16 / 16][2 Kb][4 chunks of 16 columns][16 rows][16 bytes], columns behind K zero
+ *   scales  of activations [Kb][R16], of a weight [Kb][4 ceil(N / 128)] (one byte per 32 rows); 4-byte aligned
  *
- * fdmi_quant_fp8: x [M][K] (bf16, or fp32 when x_f32) -> codes [M][ldq], scales [M][lds].  norm (optional, [K] fp32): quantises
+ * fdmi_quant_fp8: x [M][K] (bf16, or fp32 when x_f32) -> codes, scales.  norm (optional, [K] fp32): quantises
  * x * rsqrt(mean(x^2) + eps) * norm, computed in fp32 (T5LayerNorm).
- * fdmi_pack_fp8: a weight [N][K] -> codes [N][ldq], scales [ceil(N/128)][lds] and, when codes_t is given, the transposed codes
- * codes_t [K][ldqt], scales_t [ceil(K/128)][ldst] (ldqt >= N padded to 128) that an input gradient contracts with.  Padding bytes
- * of the codes are written; those of the scales are not read.                                                                       */
-int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, void* codes, int64_t ldq, void* scales, int64_t lds,
-                   int64_t M, int K, void* stream);
-int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, int64_t ldq, void* scales, int64_t lds, void* codes_t,
-                  int64_t ldqt, void* scales_t, int64_t ldst, void* stream);
+ * fdmi_pack_fp8: a weight [N][K] -> codes, scales and, when codes_t is given, those of its transpose [K][N] (the same blocks), which an
+ * input gradient contracts with.                                                                                                  */
+int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, void* codes, void* scales, int64_t M, int K,
+                   void* stream);
+int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t,
+                  void* stream);
 /* C[M][N] = act(X W^T + bias) or X W^T + bias + residual, summed in fp32, rounded once to C's type (bf16, or fp32 when out_f32; the
- * residual has C's type).  X: codes and scales as above -- or, when x is given, the unquantised activations x [M][K], and X / sx is
- * scratch of the same layout that may be written.  W2 given: the gated form; W and W2 are two weights of one shape and
- * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H [M][ldh], sh [M][ldsh] (the wi_0 / wi_1 pair of a gated feed-forward; no C, bias,
- * residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product.                                                */
+ * residual has C's type).  X / sx: codes and scales -- or, when x is given, the unquantised activations x [M][K], and X / sx is scratch of
+ * that size which may be written.  W2 given: the gated form; W and W2 are two weights of one shape and
+ * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H, sh (M rows of N columns; the wi_0 / wi_1 pair of a gated feed-forward; no C,
+ * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product.                                          */
 typedef struct fdmi_fp8_desc {
   int32_t M, N, K;
   const void* x; int64_t ldxr; int32_t x_f32;
-  void* X; int64_t ldx; void* sx; int64_t ldsx;
-  const void* W; int64_t ldw; const void* sw; int64_t ldsw;
+  void* X; void* sx;
+  const void* W; const void* sw;
   const void* W2; const void* sw2;
   const float* bias;
   const void* residual; int64_t ldr;
   void* C; int64_t ldc; int32_t out_f32; int32_t act;
-  void* H; int64_t ldh; void* sh; int64_t ldsh;
+  void* H; void* sh;
 } fdmi_fp8_desc;
 int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream);
 

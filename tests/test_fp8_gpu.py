@@ -28,6 +28,15 @@ def _np(t):
     return t.detach().double().cpu().numpy()
 
 
+def _exps(q, *a):
+    """the exponents of an operand's scales"""
+    return q.parts(*a)[1].view(torch.uint8).cpu().numpy().astype(np.int64) - 127
+
+
+def ops_untile(codes, rows, K):
+    return _ops()._untile(codes, rows, K).view(torch.uint8)
+
+
 # ---- the format --------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,K", [(1, 1), (1, 128), (2, 127), (3, 129), (5, 512), (4, 513), (17, 1155), (64, 4096), (2, 10240)])
@@ -36,8 +45,9 @@ def test_quantised_rows_are_the_formats(M, K, dtype):
     q = _ops().quant_fp8(x.cuda())
     want, exps = R.quantise(_np(x))
     assert np.array_equal(_np(q.values(F32)), want)
-    assert np.array_equal(q.scales.view(torch.uint8).cpu().numpy()[:, :exps.shape[1]].astype(np.int64) - 127, exps)
-    assert not q.codes.view(torch.uint8)[:, K:].any()                      # padding: zero codes
+    assert np.array_equal(_exps(q), exps)
+    pad = -(-K // 128) * 128
+    assert not ops_untile(q.codes, M, pad)[:, K:].any()                     # padding: zero codes
 
 
 def test_quantiser_at_the_borders_of_a_scale_and_of_a_code():
@@ -48,9 +58,9 @@ def test_quantiser_at_the_borders_of_a_scale_and_of_a_code():
     q = _ops().quant_fp8(x.cuda())
     want, exps = R.quantise(_np(x))
     # (values below 2^-126 are compared through codes and scale bytes: torch's own products of subnormals are not what is tested here)
-    codes = _np(q.codes.float())
+    codes = _np(q.parts()[0].float())
     assert np.array_equal(codes * 2.0 ** np.repeat(exps, 128, 1).astype(np.float64), want)
-    assert np.array_equal(q.scales.view(torch.uint8).cpu().numpy()[:, 0].astype(np.int64) - 127, exps[:, 0])
+    assert np.array_equal(_exps(q), exps)
 
 
 def test_all_256_codes_are_their_own_rounding_and_midpoints_go_to_even():
@@ -94,7 +104,7 @@ def _near_codes(q, ref, rel):
     by at most half a step of e4m3 (2^-4 relative, 2^-10 scales below the normal range) and that error"""
     M, K = ref.shape
     kb = -(-K // 128)
-    s = q.scales.view(torch.uint8).cpu().numpy()[:, :kb].astype(np.int64) - 127
+    s = _exps(q)
     pad = np.pad(np.abs(ref), ((0, 0), (0, kb * 128 - K))).reshape(M, kb, 128)
     amax = pad.max(2)
     sc = 2.0 ** s.astype(np.float64)
@@ -113,11 +123,10 @@ def test_packed_weight_and_its_transpose(N, K, dtype):
     p = _ops().pack_weight_fp8(w.cuda(), transposed=True)
     want, exps = R.quantise(_np(w), rows=128)
     assert np.array_equal(_np(p.values(F32)), want)
-    s = p.scales.view(torch.uint8).cpu().numpy()[:, :exps.shape[1]].astype(np.int64) - 127
-    st = p.scales_t.view(torch.uint8).cpu().numpy()[:, :exps.shape[0]].astype(np.int64) - 127
-    assert np.array_equal(s, exps) and np.array_equal(st, exps.T)
-    assert torch.equal(p.codes_t.view(torch.uint8)[:, :N], p.codes.view(torch.uint8)[:, :K].t())
-    assert not p.codes.view(torch.uint8)[:, K:].any() and not p.codes_t.view(torch.uint8)[:, N:].any()
+    assert np.array_equal(_exps(p), exps) and np.array_equal(_exps(p, True), exps.T)
+    assert torch.equal(p.parts(True)[0].view(torch.uint8), p.parts()[0].view(torch.uint8).t())
+    Kp, Np = -(-K // 128) * 128, -(-N // 128) * 128
+    assert not ops_untile(p.codes, -(-N // 16) * 16, Kp)[:, K:].any() and not ops_untile(p.codes_t, -(-K // 16) * 16, Np)[:, N:].any()
 
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------
@@ -217,7 +226,7 @@ def test_gated_product(M, N, K):
     ea, eb = R.sum_bound(K) * ma + R.pipe_bound(xv, v0), R.sum_bound(K) * mb + R.pipe_bound(xv, v1)
     e = 1.2 * ea * (np.abs(b) + eb) + (np.abs(R.gelu_tanh(a)) + 2e-6) * eb + 2e-6 * (1 + np.abs(a)) * np.abs(b)
     nb = -(-N // 128)
-    s = h.scales.view(torch.uint8).cpu().numpy()[:, :nb].astype(np.int64) - 127
+    s = _exps(h)
     pad = lambda t: np.pad(t, ((0, 0), (0, nb * 128 - N))).reshape(M, nb, 128).max(2)
     sc = 2.0 ** s.astype(np.float64)
     assert (pad(np.maximum(np.abs(ref) - e, 0)) <= 448.0 * sc).all()
@@ -226,7 +235,7 @@ def test_gated_product(M, N, K):
     got = _np(h.values(F32))
     tol = np.maximum(2.0 ** -4 * (np.abs(ref) + e), 2.0 ** -10 * full) + e
     assert (np.abs(got - ref) <= tol).all(), float((np.abs(got - ref) - tol).max())
-    assert not h.codes.view(torch.uint8)[:, N:].any()
+    assert not ops_untile(h.codes, M, nb * 128)[:, N:].any()
 
 
 def test_the_gated_feed_forward_as_a_whole():
@@ -259,7 +268,7 @@ def test_two_runs_are_bit_identical_and_a_graph_replays_them():
     def step():
         y = ops.gemm_fp8(x, W)
         h = ops.gated_fp8(ops.rmsnorm_fp8(x, None, 0.0), W, W2)
-        return y, h.codes.view(torch.uint8), h.scales.view(torch.uint8), ops.gemm_fp8_dgrad(y, W), ops.gemm_fp8(x[:3], W)
+        return y, h.values(), ops.gemm_fp8_dgrad(y, W), ops.gemm_fp8(x[:3], W)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -274,9 +283,7 @@ def test_two_runs_are_bit_identical_and_a_graph_replays_them():
         graph.replay()
         eager = step()
         torch.cuda.synchronize()
-        nb = -(-N // 128)
-        for i, (a, b) in enumerate(zip(got, eager)):
-            assert torch.equal(a[:, :nb], b[:, :nb]) if i == 2 else torch.equal(a, b)
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
 
 
 def test_refusals_on_the_gpu():

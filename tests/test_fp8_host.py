@@ -14,22 +14,21 @@ def _lib():
 
 def _desc(**kw):
     d = _lib().Fp8Desc()
-    base = dict(M=4, N=64, K=130, X=P, ldx=256, sx=P, ldsx=4, W=P, ldw=256, sw=P, ldsw=4, C=P, ldc=64)
+    base = dict(M=4, N=64, K=130, X=P, sx=P, W=P, sw=P, C=P, ldc=64)
     for k, v in {**base, **kw}.items():
         setattr(d, k, v)
     return d
 
 
+GATED = dict(W2=P, sw2=P, C=None, H=P, sh=P)
+
+
 @pytest.mark.parametrize("kw", [
-    dict(M=-1), dict(N=0), dict(K=0), dict(X=None), dict(X=P + 8), dict(ldx=128), dict(ldx=260), dict(sx=None), dict(sx=P + 2), dict(ldsx=2),
-    dict(ldsx=6), dict(W=None), dict(W=P + 4), dict(ldw=192), dict(sw=None), dict(ldsw=0), dict(C=None), dict(ldc=63), dict(act=2), dict(act=6),
-    dict(act=-1), dict(act=3, residual=P, ldr=64), dict(residual=P, ldr=63), dict(x=P, ldxr=129), dict(x=P, ldxr=130, ldx=384), dict(H=P),
-    dict(x=P, ldxr=130, ldsx=8), dict(ldw=1 << 22), dict(K=700, ldx=768, ldw=768, ldsx=4, ldsw=8),
-    # the gated form
-    dict(W2=P, sw2=P), dict(W2=P, sw2=P, C=None), dict(W2=P, C=None, H=P, ldh=128, sh=P, ldsh=4), dict(W2=P + 8, sw2=P, C=None, H=P, ldh=128, sh=P, ldsh=4),
-    dict(W2=P, sw2=P, C=None, H=P, ldh=64, sh=P, ldsh=4), dict(W2=P, sw2=P, C=None, H=P, ldh=128, sh=P, ldsh=0), dict(W2=P, sw2=P, C=None, bias=P, H=P, ldh=128, sh=P, ldsh=4),
-    dict(W2=P, sw2=P, C=None, act=5, H=P, ldh=128, sh=P, ldsh=4),
-])
+    dict(M=-1), dict(N=0), dict(K=0), dict(X=None), dict(X=P + 8), dict(sx=None), dict(sx=P + 2), dict(W=None), dict(W=P + 4), dict(sw=None),
+    dict(sw=P + 1), dict(C=None), dict(ldc=63), dict(act=2), dict(act=6), dict(act=-1), dict(act=3, residual=P, ldr=64),
+    dict(residual=P, ldr=63), dict(x=P, ldxr=129), dict(H=P), dict(sh=P), dict(K=1 << 22),
+    {**GATED, "C": P}, {**GATED, "sw2": None}, {**GATED, "W2": P + 8}, {**GATED, "H": None}, {**GATED, "H": P + 4}, {**GATED, "sh": None},
+    {**GATED, "bias": P}, {**GATED, "act": 5}, {**GATED, "residual": P, "ldr": 64}])
 def test_gemm_fp8_refuses(kw):
     L = _lib().lib()
     d = _desc(**kw)
@@ -40,24 +39,24 @@ def test_gemm_fp8_refuses(kw):
 def test_empty_calls_are_accepted_without_a_gpu():
     L = _lib().lib()
     assert L.fdmi_gemm_fp8(C.byref(_desc(M=0)), None) == 0
-    assert L.fdmi_quant_fp8(None, 0, 130, None, 0.0, None, 256, None, 4, 0, 130, None) == 0
+    assert L.fdmi_quant_fp8(None, 0, 130, None, 0.0, None, None, 0, 130, None) == 0
     assert L.fdmi_embed_fwd(None, 1, 10, 8, 8, None, 1, 0, 1.0, None, 0, 0, None, 0, None) == 0
     assert L.fdmi_embed_bwd_ws_bytes(0, 8) == 0 and L.fdmi_embed_bwd_ws_bytes(33, 8) >= 33 * 8 + 2 * 2 * 8 * 4
 
 
 @pytest.mark.parametrize("args", [
-    (None, 0, 130, None, 0.0, P, 256, P, 4, 3, 130), (P, 0, 129, None, 0.0, P, 256, P, 4, 3, 130), (P, 0, 130, None, 0.0, P, 384, P, 4, 3, 130),
-    (P, 0, 130, None, 0.0, P + 1, 256, P, 4, 3, 130), (P, 0, 130, None, 0.0, P, 256, P, 8, 3, 130), (P, 0, 130, None, 0.0, P, 256, P, 4, -3, 130),
-    (P, 0, 130, None, 0.0, P, 256, P, 4, 3, 0)])
+    (None, 0, 130, None, 0.0, P, P, 3, 130), (P, 0, 129, None, 0.0, P, P, 3, 130), (P, 0, 130, None, 0.0, P + 1, P, 3, 130),
+    (P, 0, 130, None, 0.0, None, P, 3, 130), (P, 0, 130, None, 0.0, P, P + 2, 3, 130), (P, 0, 130, None, 0.0, P, P, -3, 130),
+    (P, 0, 130, None, 0.0, P, P, 3, 0)])
 def test_quant_fp8_refuses(args):
     L = _lib().lib()
     assert L.fdmi_quant_fp8(*args, None) != 0 and b"quant_fp8" in L.fdmi_last_error()
 
 
 @pytest.mark.parametrize("args", [
-    (P, 1, 130, 0, 130, P, 256, P, 4, None, 0, None, 0), (None, 1, 130, 64, 130, P, 256, P, 4, None, 0, None, 0), (P, 1, 100, 64, 130, P, 256, P, 4, None, 0, None, 0),
-    (P, 1, 130, 64, 130, P, 130, P, 4, None, 0, None, 0), (P, 1, 130, 64, 130, P, 256, None, 4, None, 0, None, 0), (P, 1, 130, 64, 130, P, 256, P, 4, P, 64, P, 4),
-    (P, 1, 130, 64, 130, P, 256, P, 4, P, 128, None, 4)])
+    (P, 1, 130, 0, 130, P, P, None, None), (None, 1, 130, 64, 130, P, P, None, None), (P, 1, 100, 64, 130, P, P, None, None),
+    (P, 1, 130, 64, 130, P + 4, P, None, None), (P, 1, 130, 64, 130, P, None, None, None), (P, 1, 130, 64, 130, P, P, P + 8, P),
+    (P, 1, 130, 64, 130, P, P, P, None)])
 def test_pack_fp8_refuses(args):
     L = _lib().lib()
     assert L.fdmi_pack_fp8(*args, None) != 0 and b"pack_fp8" in L.fdmi_last_error()
