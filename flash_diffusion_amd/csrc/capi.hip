@@ -449,9 +449,9 @@ int fdmi_pad_cols_f32(const float* src, int cols, float* dst, int cols_pad, int6
 
 // ---- 8-bit products (fp8.hip) and the embedding lookup (embed.hip) ----
 namespace {
-// codes and scales of an 8-bit operand, the contraction short enough for 32-bit offsets into a tile of 256 rows
+// codes and scales of an 8-bit operand; contractions up to 131072 keep every segment of one at least four stages long
 bool fp8_ok(const void* codes, const void* scales, int64_t K) {
-  return codes && ((uintptr_t)codes & 15) == 0 && scales && ((uintptr_t)scales & 3) == 0 && K < (1 << 22);
+  return codes && ((uintptr_t)codes & 15) == 0 && scales && ((uintptr_t)scales & 3) == 0 && K <= (1 << 17);
 }
 }  // namespace
 
@@ -460,20 +460,20 @@ int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, flo
   FDMI_CHECK(M >= 0 && M < (1ll << 31) && K >= 1, "quant_fp8: need M >= 0 and K >= 1");
   if (M == 0) return 0;
   FDMI_CHECK(x && ldx >= K, "quant_fp8: x rows shorter than K");
-  FDMI_CHECK(fp8_ok(codes, scales, K), "quant_fp8: codes are 16-byte, scales 4-byte aligned, K < 4M");
+  FDMI_CHECK(fp8_ok(codes, scales, K), "quant_fp8: codes are 16-byte, scales 4-byte aligned, K <= 131072");
   return launch_quant_fp8(x, x_f32, ldx, norm, eps, (uint8_t*)codes, (uint8_t*)scales, M, K, (hipStream_t)stream);
 }
 int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t,
                   void* stream) {
   FDMI_CHECK(N >= 1 && K >= 1 && w && ldw >= K, "pack_fp8: need a weight [N][K]");
-  FDMI_CHECK(fp8_ok(codes, scales, K) && (!codes_t || fp8_ok(codes_t, scales_t, N)) && N < (1 << 22),
-             "pack_fp8: codes are 16-byte, scales 4-byte aligned, N and K < 4M");
+  FDMI_CHECK(fp8_ok(codes, scales, K) && (!codes_t || fp8_ok(codes_t, scales_t, N)) && N <= (1 << 17),
+             "pack_fp8: codes are 16-byte, scales 4-byte aligned, N and K <= 131072");
   return launch_pack_fp8(w, w_f32, ldw, N, K, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)codes_t, (uint8_t*)scales_t, (hipStream_t)stream);
 }
 int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
   FDMI_CHECK(d && d->M >= 0 && d->N >= 1 && d->K >= 1, "gemm_fp8: need M >= 0, N >= 1, K >= 1");
   if (d->M == 0) return 0;
-  FDMI_CHECK(fp8_ok(d->X, d->sx, d->K) && fp8_ok(d->W, d->sw, d->K), "gemm_fp8: codes are 16-byte, scales 4-byte aligned, K < 4M");
+  FDMI_CHECK(fp8_ok(d->X, d->sx, d->K) && fp8_ok(d->W, d->sw, d->K), "gemm_fp8: codes are 16-byte, scales 4-byte aligned, K <= 131072");
   FDMI_CHECK(!d->x || d->ldxr >= d->K, "gemm_fp8: x rows shorter than K");
   Fp8GemmArgs a;
   a.X = (const uint8_t*)d->X; a.sx = (const uint8_t*)d->sx;

@@ -11,7 +11,8 @@
 // Codes lie in tiles of 16 rows x 64 columns, 1 KiB each: [row tile][column tile][chunk of 16 columns][row][16 bytes].  One wave's load, store or
 // LDS transfer moves whole tiles (row-major codes fill LDS at two thirds of that rate: 128 x 128 tiles of an 8192^3 product in 627 against
 // 499 us), a matrix fragment is one 16-byte read per lane and tile, and the 16 lanes that LDS serves at once read 256 consecutive bytes.
-// Scale bytes of activations: [block of 128 columns][rows padded to 16]; of weights: [block][groups of 32 rows, padded to four groups].
+// Scale bytes of activations: [block of 128 columns][rows padded to 16]; of weights: [block][groups of 32 rows].  Weights are padded with
+// zeros to 256 rows, so a tile's loads need no bounds there.
 #include "fp8.h"
 #include "gemm.h"
 
@@ -127,9 +128,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, int64_t ldx
 // ---- weights: one workgroup per 128 x 128 block, codes in both orders (once per weight) --------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* w, int64_t ldw, int N, int K, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st) {
+  // (the grid covers both dimensions padded to 256: two blocks of 128)
   __shared__ uint8_t tile[128][132];
   __shared__ float part[4];
-  const int nb = blockIdx.y, kb = blockIdx.x, Nb = gridDim.y, Kb = gridDim.x;
+  const int nb = blockIdx.y, kb = blockIdx.x;
+  const int Nb = (N + 127) >> 7, Kb = (K + 127) >> 7, Ng = ((N + 255) >> 8) * 8, Kg = ((K + 255) >> 8) * 8;
   auto at = [&](int r, int c) {
     const int n = nb * 128 + r, k = kb * 128 + c;
     float v = 0.f;
@@ -151,8 +154,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* w, int64_t ldw, int 
     *(uint32_t*)&tile[r][c] = codes4(at(r, c), at(r, c + 1), at(r, c + 2), at(r, c + 3), up);
   }
   if (threadIdx.x < 4) {
-    s[(int64_t)kb * (Nb * 4) + nb * 4 + threadIdx.x] = (uint8_t)byte;
-    if (st) st[(int64_t)nb * (Kb * 4) + kb * 4 + threadIdx.x] = (uint8_t)byte;
+    if (kb < Kb) s[(int64_t)kb * Ng + nb * 4 + threadIdx.x] = (uint8_t)byte;
+    if (st && nb < Nb) st[(int64_t)nb * Kg + kb * 4 + threadIdx.x] = (uint8_t)byte;
   }
   __syncthreads();
   // 16-byte chunk i of the block's 16 tiles: row r, columns 16 c ..
@@ -160,13 +163,13 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* w, int64_t ldw, int 
     const int r = i & 127, c = i >> 7;
     union { uint4 v; uint8_t b[16]; } u;
     const int rt = nb * 8 + (r >> 4);
-    if (rt * 16 < N) {
+    if (kb < Kb) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) u.b[e] = tile[r][c * 16 + e];
       *(uint4*)(q + ((int64_t)rt * Kb * 2 + kb * 2 + (c >> 2)) * 1024 + (c & 3) * 256 + (r & 15) * 16) = u.v;
     }
     const int ct = kb * 8 + (r >> 4);
-    if (qt && ct * 16 < K) {
+    if (qt && nb < Nb) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) u.b[e] = tile[c * 16 + e][r];
       *(uint4*)(qt + ((int64_t)ct * Nb * 2 + nb * 2 + (c >> 2)) * 1024 + (c & 3) * 256 + (r & 15) * 16) = u.v;
@@ -247,7 +250,6 @@ __device__ __forceinline__ void store8(const Fp8GemmArgs& a, int m, int n, float
   }
 }
 __device__ __forceinline__ void store1(const Fp8GemmArgs& a, int m, int n, float v) {
-  if (m >= a.M || n >= a.N) return;
   v = act_of(a.act, a.bias ? v + a.bias[n] : v);
   if (a.out_f32) {
     if (a.residual) v += ((const float*)a.residual)[(int64_t)m * a.ldr + n];
@@ -259,67 +261,93 @@ __device__ __forceinline__ void store1(const Fp8GemmArgs& a, int m, int n, float
 }
 
 // BM x BN output tile, WM x WN waves, v_mfma_scale_f32_32x32x64 with W's rows as the first operand (lane l then holds output row l & 31 and
-// runs of four columns).  Rows past M or N repeat the last one; their results are not stored.
+// runs of four columns).
 //
 // A stage is 64 contraction steps: 64 bytes of every row, in a ring of four LDS slots filled by LDS-DMA up to three stages ahead (an
 // operand that another XCD has not touched yet comes from memory: about 2000 clocks, more than a stage's products).  A stage is MF
 // steps (32 rows of X, NF products each); the fragments of step s + AHEAD are read while step s is multiplied.  Where that reading
 // crosses into the next stage the waves hand over: the stage behind has been read by all, the next one has landed, and the slot behind
 // is refilled by pieces spread over the following steps (in one burst they would block the wave until the address unit, 64 B a
-// clock, has taken them).  The scale bytes of up to SEG blocks lie beside the ring from the start; longer contractions run in segments.
-constexpr int SEG = 96;                                              // blocks of 128 per segment
-constexpr int fp8_scale_bytes(int BM, int BN, int kb) { return kb * (BM + 8); }   // [block][BM rows of X | 8 groups of W]
-constexpr int fp8_smem(int BM, int BN, int kb) { return 4 * (BM + BN) * 64 + fp8_scale_bytes(BM, BN, kb < SEG ? kb : SEG) + 256; }   // (the last transfer of scales may be whole)
+// clock, has taken them).
+//
+// Workgroups are persistent: a work item is one tile's contraction, or one of equal segments of at most SEG blocks of a long one, and the
+// ring runs on into the next item, so a tile's epilogue is spent with the next tile's first stages on their way (a launch of one
+// workgroup per tile lost 11 us a tile at 256 x 256 x 4096).  An item's scale bytes are fetched during the item before, into the other of
+// two panels.  The last tile row is moved up to end at the last row of X; the rows it shares with its neighbour are not stored twice.
+constexpr int SEG = 48;                                              // blocks of 128 per item
+constexpr int fp8_segments(int kb) { return (kb + SEG - 1) / SEG; }
+constexpr int fp8_segment(int kb) { return (kb + fp8_segments(kb) - 1) / fp8_segments(kb); }
+// LDS: the ring, two panels of scales ([block][BM rows of X | 8 groups of W]; the last transfer into one may be whole), and what the
+// epilogue needs: a row of the gated form's maxima per wave column, or 32 x (32 NF + 1) floats per wave to turn ragged tiles round
+constexpr int fp8_panel(int BM, int kb) { return (kb < SEG ? kb : SEG) * (BM + 8) + 256; }
+constexpr int fp8_smem(int BM, int BN, int WM, int WN, bool gated, bool vec, int kb) {
+  return 4 * (BM + BN) * 64 + 2 * fp8_panel(BM, kb) + (gated ? BM * WN * 4 : vec ? 0 : WM * WN * 32 * (BN / WN + 1) * 4);
+}
 
-template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE>
-__global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArgs a, int tilesN, bool vec) {
+template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE, bool VEC>
+__global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArgs a, int tilesM, int tilesN) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NW = WM * WN, MF = BM / WM / 32, NF = BN / WN / 32, STAGE = (BM + BN) * 64;
   constexpr int AP = BM / 16 / NW, WP = BN / 16 / NW, PIECES = AP + WP;   // 1 KiB pieces (16 rows) per wave and stage
   constexpr int AHEAD = MF >= 2 ? 2 : 1, RING = 2 * MF >= 4 ? 4 : 2, BURST = (PIECES + MF - 1) / MF, LATE = AHEAD * BURST < PIECES ? AHEAD * BURST : PIECES;
-  static_assert(AP >= 1 && WP >= 1 && (!GATED || (NF == 2 && BN == 256)), "tile shape");
+  static_assert(AP >= 1 && WP >= 1 && NW % 4 == 0 && (!GATED || (NF == 2 && BN == 256 && VEC)), "tile shape");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wm = wave / WN, wn = wave % WN, half = lane >> 5, j = lane & 31;
+  const int total = tilesM * tilesN, G = gridDim.x;
+  const unsigned panel = (unsigned)a.Kb * 2048;                       // bytes of one row tile of codes
+  const int Mt = (a.M + 15) >> 4, len = fp8_segment(a.Kb);
+  const int64_t Mp = (int64_t)Mt * 16, Ng = (int64_t)((a.N + 255) >> 8) * 8;
+
   // block b runs on XCD b % 8: give each XCD a contiguous range of tiles of a column-first walk through bands of eight tile rows (the
   // tiles in flight on an XCD share eight panels of X and a few of W)
-  const int total = gridDim.x, b = blockIdx.x, xcd = b & 7, qd = total >> 3, rem = total & 7;
-  const int t = (xcd < rem ? xcd * (qd + 1) : rem * (qd + 1) + (xcd - rem) * qd) + (b >> 3);
-  const int tilesM = total / tilesN, band = t / (8 * tilesN), rows = tilesM - band * 8 < 8 ? tilesM - band * 8 : 8, in = t - band * 8 * tilesN;
-  const int m0 = (band * 8 + in % rows) * BM, n0 = (in / rows) * BN;
-
-  const unsigned panel = (unsigned)a.Kb * 2048;                       // bytes of one row tile
-  const int Mt = (a.M + 15) >> 4, Nt = (a.N + 15) >> 4;
+  struct Item { int v, m0, mt, n0, kb0, stages; };                    // mt: first row tile of X that is loaded
+  auto place = [&](Item& it) {
+    const int xcd = it.v & 7, qd = total >> 3, rem = total & 7;
+    const int t = (xcd < rem ? xcd * (qd + 1) : rem * (qd + 1) + (xcd - rem) * qd) + (it.v >> 3);
+    const int band = t / (8 * tilesN), in = t - band * 8 * tilesN, rows = tilesM - band * 8 < 8 ? tilesM - band * 8 : 8;
+    it.m0 = (band * 8 + in % rows) * BM;
+    it.n0 = (in / rows) * BN;
+    it.mt = it.m0 >> 4;
+    if (it.mt > Mt - BM / 16) it.mt = Mt > BM / 16 ? Mt - BM / 16 : 0;
+  };
+  auto cut = [&](Item& it) { it.stages = 2 * (it.kb0 + len < a.Kb ? len : a.Kb - it.kb0); };
+  auto x_of = [&](const Item& it) { return a.X + (int64_t)it.mt * panel + (int64_t)it.kb0 * 2048; };
+  // gated: the tile's rows alternate between 32 of W and the same 32 features of W2; a wave's pieces are all of one of them
+  const bool second = GATED && ((wave >> 1) & 1);
+  auto w_of = [&](const Item& it) {
+    return (second ? a.W2 : a.W) + (int64_t)(GATED ? it.n0 >> 5 : it.n0 >> 4) * panel + (int64_t)it.kb0 * 2048;
+  };
   unsigned xoff[AP], woff[WP];
-  const uint8_t* wbase[WP];
-  const uint8_t* xbase = a.X + (int64_t)(m0 >> 4) * panel;
 #pragma unroll
   for (int p = 0; p < AP; ++p) {
     const int r = p * NW + wave;
-    xoff[p] = (unsigned)((m0 >> 4) + r < Mt ? r : Mt - 1 - (m0 >> 4)) * panel + lane * 16;
+    xoff[p] = (unsigned)(r < Mt ? r : Mt - 1) * panel + lane * 16;
   }
 #pragma unroll
   for (int p = 0; p < WP; ++p) {
     const int r = p * NW + wave;
-    if (GATED) {   // tile rows alternate between 32 of W and the same 32 features of W2
-      const int f0 = n0 >> 5, f = (r >> 2) * 2 + (r & 1);
-      wbase[p] = ((r >> 1) & 1 ? a.W2 : a.W) + (int64_t)f0 * panel;
-      woff[p] = (unsigned)(f0 + f < Nt ? f : Nt - 1 - f0) * panel + lane * 16;
-    } else {
-      wbase[p] = a.W + (int64_t)(n0 >> 4) * panel;
-      woff[p] = (unsigned)((n0 >> 4) + r < Nt ? r : Nt - 1 - (n0 >> 4)) * panel + lane * 16;
-    }
+    woff[p] = (unsigned)(GATED ? (r >> 2) * 2 + (r & 1) : r) * panel + lane * 16;
   }
+
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
-  const int stages = a.Kb * 2;
-  // piece p of stage h.  A stage past the end repeats the last one (the count of transfers in flight stays the same; nothing reads it)
-  auto piece = [&](int h, int p) {
-    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(lds0 + (h & 3) * STAGE + wave * 1024);
-    const int64_t k = (int64_t)(h < stages ? h : stages - 1) * 1024;
-    if (p < AP) dma16(xbase + k, xoff[p < AP ? p : 0], to + p * NW * 1024);
-    else dma16(wbase[p < AP ? 0 : p - AP] + k, woff[p < AP ? 0 : p - AP], to + BM * 64 + (p - AP) * NW * 1024);
+  const int panel_bytes = fp8_panel(BM, a.Kb);
+  auto fetch_scales = [&](const Item& it, int which) {                // four bytes per lane, 64 lanes per transfer
+    constexpr int per = BM / 4 + 2;
+    const int count = (it.stages >> 1) * per;
+    for (int e0 = wave * 64; e0 < count; e0 += NW * 64) {
+      const int e = e0 + lane < count ? e0 + lane : count - 1, kb = e / per, r = e - kb * per;
+      const uint8_t* src;
+      if (r < BM / 4) {
+        const int64_t m = (int64_t)it.mt * 16 + r * 4;
+        src = a.sx + (it.kb0 + kb) * Mp + (m < Mp ? m : Mp - 4);
+      } else {
+        const int64_t g = GATED ? (it.n0 >> 8) * 4 : (it.n0 >> 7) * 4 + (r - BM / 4) * 4;
+        src = (GATED && r > BM / 4 ? a.sw2 : a.sw) + (it.kb0 + kb) * Ng + (g < Ng ? g : Ng - 4);
+      }
+      dma4(src, (unsigned)__builtin_amdgcn_readfirstlane(lds0 + 4 * STAGE + which * panel_bytes + e0 * 4));
+    }
   };
 
-  const int half = lane >> 5, j = lane & 31;
   f32x16 acc[NF][MF];
 #pragma unroll
   for (int i = 0; i < NF; ++i)
@@ -328,17 +356,16 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
   i32x8 x[RING], w[2][NF];
   mfma_b8 wide[WIDE ? NF : 1][4];
   int sx[MF], sw[NF], nsx[MF], nsw[NF];
-  auto frag = [&](int h, int row) {               // rows row + (0 .. 31), columns 32 half + (0 .. 31) of stage h
-    const char* r = smem + (h & 3) * STAGE + row * 64 + (j >> 4) * 1024 + half * 512 + (j & 15) * 16;
+  auto frag = [&](int slot, int row) {            // rows row + (0 .. 31), columns 32 half + (0 .. 31) of a stage
+    const char* r = smem + (slot & 3) * STAGE + row * 64 + (j >> 4) * 1024 + half * 512 + (j & 15) * 16;
     return join(*(const uint4*)r, *(const uint4*)(r + 256));
   };
-  auto read_step = [&](int kb, int s) {          // s counts through the two stages of block kb (and on into the next block)
-    const int h = 2 * kb + s / MF;
+  auto read_step = [&](int slot, int s) {         // step s of the two stages of a block, and on into the next block's
     if (s % MF == 0) {
 #pragma unroll
-      for (int i = 0; i < NF; ++i) w[s / MF & 1][i] = frag(h, BM + wn * (BN / WN) + i * 32);
+      for (int i = 0; i < NF; ++i) w[s / MF & 1][i] = frag(slot + s / MF, BM + wn * (BN / WN) + i * 32);
     }
-    x[s % RING] = frag(h, wm * (BM / WM) + (s % MF) * 32);
+    x[s % RING] = frag(slot + s / MF, wm * (BM / WM) + (s % MF) * 32);
   };
   auto multiply = [&](int s) {
     const int k = s % MF, ks = s / MF;
@@ -361,76 +388,61 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
       }
     }
   };
-  // scale bytes of block kb of this segment.  W's eight bytes: four 32-row groups from its first operand, four from the next four groups
-  // or, gated, from W2 (a 64-row tile finds its two groups at the place they have among four)
-  const char* sbase = smem + 4 * STAGE;
-  auto read_scales = [&](int kb) {
-    const char* q = sbase + kb * (BM + 8);
+  // scale bytes of an item's block kb.  W's eight bytes: four 32-row groups of W, then the next four or, gated, those of W2
+  auto read_scales = [&](const Item& it, int which, int kb) {
+    const char* q = smem + 4 * STAGE + which * panel_bytes + kb * (BM + 8);
 #pragma unroll
     for (int i = 0; i < MF; ++i) nsx[i] = *(const uint8_t*)(q + wm * (BM / WM) + i * 32 + j);
 #pragma unroll
-    for (int i = 0; i < NF; ++i) nsw[i] = *(const uint8_t*)(q + BM + (GATED ? i * 4 + wn : (BN < 128 ? (n0 >> 5) & 3 : 0) + wn * NF + i));
+    for (int i = 0; i < NF; ++i) nsw[i] = *(const uint8_t*)(q + BM + (GATED ? i * 4 + wn : (BN < 128 ? (it.n0 >> 5) & 3 : 0) + wn * NF + i));
   };
 
-  for (int seg = 0; seg < a.Kb; seg += SEG) {
-    const int end = seg + SEG < a.Kb ? seg + SEG : a.Kb;
-    if (seg) {                                    // the ring and the scales of the segment behind are free
-      dma_wait<0>();
-      __builtin_amdgcn_s_barrier();
-    }
-    const int per = BM / 4 + 2, count = (end - seg) * per;                      // four bytes per lane, 64 lanes per transfer
-    const int64_t Mp = (int64_t)Mt * 16, Ng = (int64_t)((a.N + 127) >> 7) * 4;
-    for (int e0 = wave * 64; e0 < count; e0 += NW * 64) {
-      const int e = e0 + lane < count ? e0 + lane : count - 1, kb = e / per, r = e - kb * per;
-      const uint8_t* src;
-      if (r < BM / 4) src = a.sx + (seg + kb) * Mp + (m0 + r * 4 < Mp ? m0 + r * 4 : Mp - 4);
-      else {
-        const int64_t g = GATED ? (n0 >> 8) * 4 : (n0 >> 7) * 4 + (r - BM / 4) * 4;
-        src = (GATED && r > BM / 4 ? a.sw2 : a.sw) + (seg + kb) * Ng + (g < Ng ? g : Ng - 4);
-      }
-      dma4(src, (unsigned)__builtin_amdgcn_readfirstlane(lds0 + 4 * STAGE + e0 * 4));
-    }
-    const int h0 = 2 * seg;
+  auto epilogue = [&](const Item& it) {
+    const int mw = it.mt * 16 + wm * (BM / WM), nw = it.n0 + wn * (BN / WN);
+    if constexpr (GATED) {
+      // the tile's 128 features are one block of the next product's contraction: amax per row over the four waves of a row group
+      float* red = (float*)(smem + 4 * STAGE + 2 * panel_bytes);      // [BM][WN]
+      float h[MF][16];
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
+      for (int k = 0; k < MF; ++k) {
+        float m = 0.f;
 #pragma unroll
-      for (int p = 0; p < (h < 3 ? PIECES : LATE); ++p) piece(h0 + h, p);   // (the loop's first steps issue the rest of the fourth)
-    dma_wait<2 * PIECES + LATE>();                                          // (the scales are older: landed too)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read_scales(0);
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) read_step(seg, s);
-    for (int kb = seg; kb < end; ++kb) {          // (no branch in this body: the compiler would sink the products past it)
-#pragma unroll
-      for (int i = 0; i < MF; ++i) sx[i] = nsx[i];
-#pragma unroll
-      for (int i = 0; i < NF; ++i) sw[i] = nsw[i];
-#pragma unroll
-      for (int s = 0; s < 2 * MF; ++s) {
-        if (s % MF == MF - AHEAD) {               // hand over
-          dma_wait<2 * PIECES>();
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
+        for (int r = 0; r < 16; ++r) {
+          const int f = it.n0 / 2 + wn * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+          h[k][r] = f < a.N ? gelu_tanh_fast(acc[0][k][r]) * acc[1][k][r] : 0.f;
+          m = fmaxf(m, finite_abs(h[k][r]));
         }
-        read_step(kb, s + AHEAD);
-        if (s == 0) read_scales((kb + 1 < end ? kb + 1 : kb) - seg);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(s);
-        __builtin_amdgcn_sched_barrier(0);
-        const int u = (s + AHEAD) % MF, h = 2 * kb + (s + AHEAD) / MF + 3;   // burst u since the hand-over to stage h - 3
-#pragma unroll
-        for (int p = u * BURST; p < (u + 1) * BURST && p < PIECES; ++p) piece(h, p);
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if (half == 0) red[(wm * (BM / WM) + k * 32 + j) * WN + wn] = m;
       }
-    }
-  }
-
-  if constexpr (!GATED) {
-    const int mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
-    if (vec && nw + NF * 32 <= a.N) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < MF; ++k) {
+        const int row = wm * (BM / WM) + k * 32 + j, m = it.mt * 16 + row;
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < WN; ++i) mx = fmaxf(mx, red[row * WN + i]);
+        const int byte = scale_byte(mx);
+        const float up = scale_up(byte);
+        uint32_t d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[r] = codes4(h[k][4 * r], h[k][4 * r + 1], h[k][4 * r + 2], h[k][4 * r + 3], up);
+        // lanes l and l + 32 hold alternating runs of four features: exchange so that each has 16 consecutive ones
+        const auto e0 = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
+        const auto e1 = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+        if (m >= it.m0 && m < a.M) {
+          const int nb = (a.N + 127) >> 7, blk = it.n0 >> 8;
+          *(uint4*)(a.H + ((int64_t)(m >> 4) * nb * 2 + blk * 2 + (wn >> 1)) * 1024 + ((wn & 1) * 2 + half) * 256 + (m & 15) * 16) =
+              make_uint4(e0[0], e0[1], e1[0], e1[1]);
+          if (half == 0 && wn == 0) a.sh[(int64_t)blk * Mp + m] = (uint8_t)byte;
+        }
+      }
+      __syncthreads();                                                // (red is written again by the next tile)
+    } else if constexpr (VEC) {
       // lanes l and l + 32 hold alternating runs of four columns: exchange so that each has eight consecutive ones
 #pragma unroll
-      for (int k = 0; k < MF; ++k)
+      for (int k = 0; k < MF; ++k) {
+        const int m = mw + k * 32 + j;
 #pragma unroll
         for (int i = 0; i < NF; ++i)
 #pragma unroll
@@ -443,76 +455,232 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
               v[t] = __uint_as_float(e[0]);
               v[4 + t] = __uint_as_float(e[1]);
             }
-            if (mw + k * 32 + j < a.M) store8(a, mw + k * 32 + j, nw + i * 32 + r * 16 + half * 8, v);
+            const int n = nw + i * 32 + r * 16 + half * 8;
+            if (m >= it.m0 && m < a.M && n < a.N) store8(a, m, n, v);
           }
+      }
     } else {
-      // ragged or unaligned: each wave turns 32 rows at a time round in LDS and stores single columns
-      dma_wait<0>();
-      __syncthreads();
+      // rows of C that are not aligned: each wave turns 32 rows at a time round in LDS and stores single columns
       constexpr int LD = NF * 32 + 1;
-      float* turn = (float*)smem + wave * 32 * LD;
+      float* turn = (float*)(smem + 4 * STAGE + 2 * panel_bytes) + wave * 32 * LD;
 #pragma unroll
       for (int k = 0; k < MF; ++k) {
 #pragma unroll
         for (int i = 0; i < NF; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) turn[j * LD + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3)] = acc[i][k][r];
-        for (int e = lane; e < 32 * NF * 32; e += 64) store1(a, mw + k * 32 + e / (NF * 32), nw + e % (NF * 32), turn[e / (NF * 32) * LD + e % (NF * 32)]);
+        for (int e = lane; e < 32 * NF * 32; e += 64) {
+          const int m = mw + k * 32 + e / (NF * 32), n = nw + e % (NF * 32);
+          if (m >= it.m0 && m < a.M && n < a.N) store1(a, m, n, turn[e / (NF * 32) * LD + e % (NF * 32)]);
+        }
       }
     }
-  } else {
-    // the tile's 128 features are one block of the next product's contraction: amax per row over the four waves of a row group
-    float* red = (float*)smem;                                        // [BM][WN]
-    dma_wait<0>();
-    __syncthreads();
-    float h[MF][16];
 #pragma unroll
-    for (int k = 0; k < MF; ++k) {
-      float m = 0.f;
+    for (int i = 0; i < NF; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int f = n0 / 2 + wn * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        h[k][r] = f < a.N ? gelu_tanh_fast(acc[0][k][r]) * acc[1][k][r] : 0.f;
-        m = fmaxf(m, finite_abs(h[k][r]));
-      }
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      if (half == 0) red[(wm * (BM / WM) + k * 32 + j) * WN + wn] = m;
+      for (int k = 0; k < MF; ++k) acc[i][k] = (f32x16){};
+  };
+
+  Item cur;
+  cur.v = blockIdx.x;
+  cur.kb0 = 0;
+  place(cur);
+  cut(cur);
+  int slot = 0, which = 0;                        // ring position of the item's first stage; its panel
+  const uint8_t* xb = x_of(cur);
+  const uint8_t* wb = w_of(cur);
+  auto piece_at = [&](const uint8_t* xk, const uint8_t* wk, int at, int p) {
+    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(lds0 + (at & 3) * STAGE + wave * 1024);
+    if (p < AP) dma16(xk, xoff[p < AP ? p : 0], to + p * NW * 1024);
+    else dma16(wk, woff[p < AP ? 0 : p - AP], to + BM * 64 + (p - AP) * NW * 1024);
+  };
+  fetch_scales(cur, 0);
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+#pragma unroll
+    for (int p = 0; p < (h < 3 ? PIECES : LATE); ++p) {    // (the loop's first steps issue the rest of the fourth)
+      const int64_t k = (int64_t)(h < cur.stages ? h : cur.stages - 1) * 1024;
+      piece_at(xb + k, wb + k, h, p);
     }
-    __syncthreads();
+  dma_wait<2 * PIECES + LATE>();                  // (the scales are older: landed too)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < MF; ++k) {
-      const int row = wm * (BM / WM) + k * 32 + j, m = m0 + row;
-      float mx = 0.f;
+  for (int s = 0; s < AHEAD; ++s) read_step(0, s);
+  while (true) {
+    Item nxt = cur;
+    nxt.kb0 += len;
+    bool more = nxt.kb0 < a.Kb;
+    const bool done = !more;                      // the tile ends with this item
+    if (done) {
+      nxt.kb0 = 0;
+      nxt.v += G;
+      more = nxt.v < total;
+      if (more) place(nxt);
+    }
+    // where the stages behind this item's lie: the next item's, or its own last one over and over
+    int64_t xd = (int64_t)(cur.stages - 1) * 1024, wd = xd;
+    int step = 0;
+    if (more) {
+      cut(nxt);
+      fetch_scales(nxt, which ^ 1);
+      xd = x_of(nxt) - xb;
+      wd = w_of(nxt) - wb;
+      step = 1024;
+    }
+    read_scales(cur, which, 0);
+    const int blocks = cur.stages >> 1;
+    for (int kb = 0; kb < blocks; ++kb) {         // (no branch in this body: the compiler would sink the products past it)
 #pragma unroll
-      for (int i = 0; i < WN; ++i) mx = fmaxf(mx, red[row * WN + i]);
-      const int byte = scale_byte(mx);
-      const float up = scale_up(byte);
-      uint32_t d[4];
+      for (int i = 0; i < MF; ++i) sx[i] = nsx[i];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) d[r] = codes4(h[k][4 * r], h[k][4 * r + 1], h[k][4 * r + 2], h[k][4 * r + 3], up);
-      // lanes l and l + 32 hold alternating runs of four features: exchange so that each has 16 consecutive ones
-      const auto e0 = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
-      const auto e1 = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
-      if (m < a.M) {
-        const int nb = (a.N + 127) >> 7, blk = n0 >> 8;
-        *(uint4*)(a.H + ((int64_t)(m >> 4) * nb * 2 + blk * 2 + (wn >> 1)) * 1024 + ((wn & 1) * 2 + half) * 256 + (m & 15) * 16) =
-            make_uint4(e0[0], e0[1], e1[0], e1[1]);
-        if (half == 0 && wn == 0) a.sh[(int64_t)blk * Mt * 16 + m] = (uint8_t)byte;
+      for (int i = 0; i < NF; ++i) sw[i] = nsw[i];
+#pragma unroll
+      for (int s = 0; s < 2 * MF; ++s) {
+        if (s % MF == MF - AHEAD) {               // hand over
+          dma_wait<2 * PIECES>();
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        read_step(slot + 2 * kb, s + AHEAD);
+        if (s == 0) read_scales(cur, which, kb + 1 < blocks ? kb + 1 : kb);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s);
+        __builtin_amdgcn_sched_barrier(0);
+        const int u = (s + AHEAD) % MF, h = 2 * kb + (s + AHEAD) / MF + 3;   // burst u since the hand-over to stage h - 3
+        const int over = h - cur.stages;
+        const int64_t in = over >> 31, own = (int64_t)h * 1024, far = (int64_t)over * step;
+        const int64_t kx = (in & own) | (~in & (xd + far)), kw = (in & own) | (~in & (wd + far));
+#pragma unroll
+        for (int p = u * BURST; p < (u + 1) * BURST && p < PIECES; ++p) piece_at(xb + kx, wb + kw, slot + h, p);
+      }
+    }
+    if (done) epilogue(cur);
+    if (!more) break;
+    slot += cur.stages;
+    which ^= 1;
+    cur = nxt;
+    xb = x_of(cur);
+    wb = w_of(cur);
+  }
+  dma_wait<0>();                                  // no transfer may be on its way when the workgroup's LDS is released
+}
+
+template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE, bool VEC>
+int launch_tile(const Fp8GemmArgs& a, hipStream_t st) {
+  constexpr int most = fp8_smem(BM, BN, WM, WN, GATED, VEC, SEG);
+  static_assert(most <= 160 * 1024, "LDS");
+  FDMI_HIP(hipFuncSetAttribute((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, most));
+  const int smem = fp8_smem(BM, BN, WM, WN, GATED, VEC, a.Kb);
+  const int64_t tilesM = ((int64_t)a.M + BM - 1) / BM, tilesN = ((int64_t)a.N * (GATED ? 2 : 1) + BN - 1) / BN;
+  FDMI_CHECK(tilesM * tilesN < (1ll << 30), "gemm_fp8: too many tiles");
+  // as many workgroups as fit (a multiple of the 8 XCDs); one per tile where an item is too short for the ring to run across items
+  int fit = 160 * 1024 / smem;
+  if (fit > 2048 / (WM * WN * 64)) fit = 2048 / (WM * WN * 64);
+  const int64_t room = (int64_t)256 * fit, total = tilesM * tilesN;
+  const int64_t grid = a.Kb < 2 || total < room ? total : room;
+  hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE, VEC>), dim3((unsigned)grid), dim3(WM * WN * 64), smem, st, a, (int)tilesM,
+                     (int)tilesN);
+  FDMI_HIP(hipGetLastError());
+  return 0;
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------------------------
+// A product of few rows is bound by streaming the weight once.  A workgroup takes 16 NT rows of W and 16 MT rows of X; its eight waves share
+// out the contraction (block kb goes to wave kb % 8), fetch whole tiles straight into matrix fragments -- a lane's two 16-byte reads of
+// a 16 x 128 pair of tiles are v_mfma_scale_f32_16x16x128's operand -- DEPTH blocks at a time, and join their sums through LDS in the
+// order of the waves.  No split over workgroups: N / 16 of them fill the chip from N = 4096 on, and smaller weights sit in L2.
+constexpr int fp8_stream_smem(int MT, int NT) { return 8 * MT * 16 * (NT * 16 + 4) * 4; }
+
+template <int MT, int NT, bool WIDE>
+__global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int DEPTH = MT * 2 + NT * 2 <= 4 ? 4 : MT * 2 + NT * 2 <= 8 ? 2 : 1, LD = NT * 16 + 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t panel = (int64_t)a.Kb * 2048;
+  const int Mt = (a.M + 15) >> 4, mt0 = blockIdx.y * MT, nt0 = blockIdx.x * NT;
+  const int64_t Mp = (int64_t)Mt * 16, Ng = (int64_t)((a.N + 255) >> 8) * 8;
+  const uint8_t* wp[NT];
+  const uint8_t* xp[MT];
+  const uint8_t* sxp[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) wp[i] = a.W + (nt0 + i) * panel + lane * 16;
+#pragma unroll
+  for (int k = 0; k < MT; ++k) {
+    const int mt = mt0 + k < Mt ? mt0 + k : Mt - 1;                  // (rows past the last tile repeat it and are not stored)
+    xp[k] = a.X + mt * panel + lane * 16;
+    sxp[k] = a.sx + mt * 16 + (lane & 15);
+  }
+  const uint8_t* swp = a.sw + (nt0 >> 1);
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int k = 0; k < MT; ++k) acc[i][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int kb0 = wave; kb0 < a.Kb; kb0 += 8 * DEPTH) {
+    i32x8 w[DEPTH][NT], x[DEPTH][MT];
+    int sw[DEPTH], sx[DEPTH][MT];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int kb = kb0 + 8 * d < a.Kb ? kb0 + 8 * d : kb0;
+      const int64_t o = (int64_t)kb * 2048;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) w[d][i] = join(*(const uint4*)(wp[i] + o), *(const uint4*)(wp[i] + o + 1024));
+#pragma unroll
+      for (int k = 0; k < MT; ++k) x[d][k] = join(*(const uint4*)(xp[k] + o), *(const uint4*)(xp[k] + o + 1024));
+      sw[d] = swp[kb * Ng];                                            // (16 NT rows lie in one group of 32)
+#pragma unroll
+      for (int k = 0; k < MT; ++k) sx[d][k] = sxp[k][kb * Mp];
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (kb0 + 8 * d >= a.Kb) break;
+      if constexpr (!WIDE) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int k = 0; k < MT; ++k)
+            acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[d][i], x[d][k], acc[i][k], 0, 0, 0, sw[d], 0, sx[d][k]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          mfma_b8 wb[NT];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) wb[i] = widen8(w[d][i][2 * q], w[d][i][2 * q + 1], scale_of(sw[d]));
+#pragma unroll
+          for (int k = 0; k < MT; ++k) {
+            const mfma_b8 xb = widen8(x[d][k][2 * q], x[d][k][2 * q + 1], scale_of(sx[d][k]));
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[i], xb, acc[i][k], 0, 0, 0);
+          }
+        }
       }
     }
   }
+  // lane l holds output row l & 15 and columns 4 (l >> 4) + 0 .. 3 of each fragment
+  float* red = (float*)smem;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int k = 0; k < MT; ++k)
+      *(f32x4*)(red + ((wave * MT + k) * 16 + (lane & 15)) * LD + i * 16 + (lane >> 4) * 4) = acc[i][k];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MT * 16 * NT * 16; e += 512) {
+    const int r = e / (NT * 16), c = e % (NT * 16), m = mt0 * 16 + r, n = nt0 * 16 + c;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += red[(q * MT * 16 + r) * LD + c];
+    if (m < a.M && n < a.N) store1(a, m, n, v);
+  }
 }
 
-template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE>
-int launch_tile(const Fp8GemmArgs& a, bool vec, hipStream_t st) {
-  constexpr int most = fp8_smem(BM, BN, SEG);
-  static_assert(most <= 160 * 1024, "LDS");
-  FDMI_HIP(hipFuncSetAttribute((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, most));
-  const int smem = fp8_smem(BM, BN, a.Kb);
-  const int64_t tilesM = ((int64_t)a.M + BM - 1) / BM, tilesN = ((int64_t)a.N * (GATED ? 2 : 1) + BN - 1) / BN;
-  FDMI_CHECK(tilesM * tilesN < (1ll << 31), "gemm_fp8: too many tiles");
-  hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>), dim3((unsigned)(tilesM * tilesN)), dim3(WM * WN * 64), smem, st, a, (int)tilesN,
-                     vec);
+template <int MT, int NT, bool WIDE>
+int launch_stream(const Fp8GemmArgs& a, hipStream_t st) {
+  constexpr int smem = fp8_stream_smem(MT, NT);
+  static_assert(smem <= 160 * 1024, "LDS");
+  FDMI_HIP(hipFuncSetAttribute((const void*)fp8_stream_kernel<MT, NT, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const dim3 grid(cdiv(a.N, NT * 16), cdiv(a.M, MT * 16));
+  hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE>), grid, dim3(512), smem, st, a);
   FDMI_HIP(hipGetLastError());
   return 0;
 }
@@ -538,21 +706,55 @@ int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, f
 }
 
 int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st, hipStream_t stream) {
-  const dim3 grid(cdiv(K, 128), cdiv(N, 128));
+  const dim3 grid(qt ? cdiv(K, 256) * 2 : cdiv(K, 128), cdiv(N, 256) * 2);
   if (w_f32) hipLaunchKernelGGL(pack_kernel<float>, grid, dim3(256), 0, stream, (const float*)w, ldw, N, K, q, s, qt, st);
   else hipLaunchKernelGGL(pack_kernel<bf16_t>, grid, dim3(256), 0, stream, (const bf16_t*)w, ldw, N, K, q, s, qt, st);
   FDMI_HIP(hipGetLastError());
   return 0;
 }
 
+// Which kernel: the least of the times measured for each, as a function of the problem (microseconds).  A tile kernel spends `block` + `share` * w
+// on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU rounded up; the streaming kernel is bound by what its workgroups
+// read from L2 (25 TB/s over all CUs; a short grid leaves some idle) or by the weight from memory.  Measured against each other at
+// 8192^3, 1920 x 4096 x {4096, 10240}, {1, 16, 64} x 4096 x 4096, 512 x 1024 x 4096, 120 x 1024 x 2560, 2048 x 2048 x 4096, for example
+// (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 18.4 / 22.9 / -, 4.3;  1920 x 4096 x 4096: 51 / 34.4 / 33.8 / 50, 91;
+// 16384 x 10240 x 4096: 1020 / 626 / 588 / 534, -.
+struct Fp8Cost { int BM, BN; double block, share, fixed, tile; };
+double fp8_cost(const Fp8GemmArgs& a, const Fp8Cost& c) {
+  const double tiles = double((a.M + c.BM - 1) / c.BM) * ((a.N + c.BN - 1) / c.BN), w = (double)(int64_t)((tiles + 255) / 256);
+  return c.fixed + c.tile * w + a.Kb * (c.block + c.share * w);
+}
+double fp8_stream_cost(const Fp8GemmArgs& a, int rows) {   // `rows` rows of X and of W per workgroup
+  double groups = double((a.M + rows - 1) / rows) * ((a.N + rows - 1) / rows);
+  if (groups < 256) groups = 256;
+  const double l2 = groups * 2 * rows * a.Kb * 128 / 25e6, hbm = double(a.N) * a.Kb * 128 / 4.5e6;
+  return 2.7 + (l2 > hbm ? l2 : hbm);
+}
+
 int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st) {
   if (a.M == 0) return 0;
+  if (a.H) return a.M <= 64 ? launch_tile<64, 256, 1, 4, true, false, true>(a, st) : launch_tile<128, 256, 2, 4, true, false, true>(a, st);
   const int es = a.out_f32 ? 4 : 2;
-  const bool vec = a.H || (aligned(a.C, a.ldc * es, 16) && (!a.residual || aligned(a.residual, a.ldr * es, 16)) && ((uintptr_t)a.bias & 15) == 0);
-  if (a.H) return a.M <= 64 ? launch_tile<64, 256, 1, 4, true, false>(a, vec, st) : launch_tile<128, 256, 2, 4, true, false>(a, vec, st);
-  const int64_t big = ((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128);
-  if (a.out_f32) return big < 256 ? launch_tile<64, 64, 2, 2, false, true>(a, vec, st) : launch_tile<128, 128, 2, 2, false, true>(a, vec, st);
-  if (big < 256) return launch_tile<64, 64, 2, 2, false, false>(a, vec, st);
-  if (big < 2048) return launch_tile<128, 128, 2, 2, false, false>(a, vec, st);
-  return launch_tile<256, 256, 2, 4, false, false>(a, vec, st);
+  const bool vec = a.N % 8 == 0 && aligned(a.C, a.ldc * es, 16) && (!a.residual || aligned(a.residual, a.ldr * es, 16)) && ((uintptr_t)a.bias & 15) == 0;
+  static const Fp8Cost narrow[] = {{64, 64, .09, .172, 3., .5}, {128, 128, .02, .46, 3., 1.}, {128, 256, 0., .86, 3., 3.}, {256, 256, 0., 1.45, 3., 5.}};
+  static const Fp8Cost wide[] = {{64, 64, .20, .25, 3., .5}, {128, 128, .13, .80, 3., 1.}, {256, 256, 0., 3., 3., 5.}};
+  const Fp8Cost* table = a.out_f32 ? wide : narrow;
+  int best = -1;
+  double least = 0.;
+  for (int i = 0; i < (a.out_f32 ? 3 : 4); ++i) {
+    if (table[i].BN > 128 && !vec) continue;               // (no room in LDS to turn ragged tiles round)
+    const double c = fp8_cost(a, table[i]);
+    if (best < 0 || c < least) { best = i; least = c; }
+  }
+  const double s16 = fp8_stream_cost(a, 16), s32 = fp8_stream_cost(a, 32);
+  if (s16 <= s32 && s16 < least) return a.out_f32 ? launch_stream<1, 1, true>(a, st) : launch_stream<1, 1, false>(a, st);
+  if (s32 < least) return a.out_f32 ? launch_stream<2, 2, true>(a, st) : launch_stream<2, 2, false>(a, st);
+#define FP8_TILE(BM, BN, WM, WN, WIDE) (vec ? launch_tile<BM, BN, WM, WN, false, WIDE, true>(a, st) : launch_tile<BM, BN, WM, WN, false, WIDE, false>(a, st))
+  switch (table[best].BM + table[best].BN) {
+    case 128: return a.out_f32 ? FP8_TILE(64, 64, 2, 2, true) : FP8_TILE(64, 64, 2, 2, false);
+    case 256: return a.out_f32 ? FP8_TILE(128, 128, 2, 2, true) : FP8_TILE(128, 128, 2, 2, false);
+    case 384: return launch_tile<128, 256, 2, 4, false, false, true>(a, st);
+    default: return a.out_f32 ? launch_tile<256, 256, 2, 4, false, true, true>(a, st) : launch_tile<256, 256, 2, 4, false, false, true>(a, st);
+  }
+#undef FP8_TILE
 }

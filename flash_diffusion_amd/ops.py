@@ -492,15 +492,15 @@ class Fp8Weight:
 
     def __init__(self, N, K, device, transposed):
         self.N, self.K = N, K
-        new = lambda n, k: (torch.empty(_pad(n, 16) * _pad(k, 128), dtype=torch.uint8, device=device),
-                            torch.empty(_pad(k, 128) // 128 * (_pad(n, 128) // 32), dtype=torch.uint8, device=device))
+        new = lambda n, k: (torch.empty(_pad(n, 256) * _pad(k, 128), dtype=torch.uint8, device=device),
+                            torch.empty(_pad(k, 128) // 128 * (_pad(n, 256) // 32), dtype=torch.uint8, device=device))
         self.codes, self.scales = new(N, K)
         self.codes_t, self.scales_t = new(K, N) if transposed else (None, None)
 
     def parts(self, transposed=False):
         """(codes [N, K] e4m3, scales [ceil(N / 128), ceil(K / 128)] e8m0), or those of the transpose"""
         n, k, c, s = (self.K, self.N, self.codes_t, self.scales_t) if transposed else (self.N, self.K, self.codes, self.scales)
-        return _untile(c, n, k), s.view(_pad(k, 128) // 128, -1)[:, ::4].t().contiguous().view(E8)
+        return _untile(c, n, k), s.view(_pad(k, 128) // 128, -1)[:, ::4][:, :_pad(n, 128) // 128].t().contiguous().view(E8)
 
     def values(self, dtype=F32):
         c, s = self.parts()

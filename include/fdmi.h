@@ -210,9 +210,9 @@ int fdmi_dmd_loss(const float* s, const float* noisy, const float* real, const f
  * The frozen text encoders' linears (T5-XXL behind embedders/t5/t5_embedder_model.py:11-104) in 8 bits: codes are e4m3, a scale is
  * a power of two held as its biased exponent in one byte (e8m0), 2^e the smallest power with amax <= 448 2^e over the block.  A row of
  * activations has one scale per 128 columns, a weight [N][K] one per 128 x 128 block.  An infinity or NaN becomes the NaN code and does
- * not enter its block's scale.  Kb = ceil(K / 128), R16 = rows padded to 16:
- *   codes   R16 * Kb * 128 bytes, 16-byte aligned: tiles [R16 / 16][2 Kb][4 chunks of 16 columns][16 rows][16 bytes], columns behind K zero
- *   scales  of activations [Kb][R16], of a weight [Kb][4 ceil(N / 128)] (one byte per 32 rows); 4-byte aligned
+ * not enter its block's scale.  Kb = ceil(K / 128), K <= 131072; R = rows padded to 16 (activations) or 256 (weights):
+ *   codes   R * Kb * 128 bytes, 16-byte aligned: tiles [R / 16][2 Kb][4 chunks of 16 columns][16 rows][16 bytes], columns behind K zero
+ *   scales  of activations [Kb][R], of a weight [Kb][R / 32] (one byte per 32 rows); 4-byte aligned
  *
  * fdmi_quant_fp8: x [M][K] (bf16, or fp32 when x_f32) -> codes, scales.  norm (optional, [K] fp32): quantises
  * x * rsqrt(mean(x^2) + eps) * norm, computed in fp32 (T5LayerNorm).

@@ -125,8 +125,10 @@ def test_packed_weight_and_its_transpose(N, K, dtype):
     assert np.array_equal(_np(p.values(F32)), want)
     assert np.array_equal(_exps(p), exps) and np.array_equal(_exps(p, True), exps.T)
     assert torch.equal(p.parts(True)[0].view(torch.uint8), p.parts()[0].view(torch.uint8).t())
-    Kp, Np = -(-K // 128) * 128, -(-N // 128) * 128
-    assert not ops_untile(p.codes, -(-N // 16) * 16, Kp)[:, K:].any() and not ops_untile(p.codes_t, -(-K // 16) * 16, Np)[:, N:].any()
+    up = lambda n, to: -(-n // to) * to                                  # padding: zero codes
+    for c, n, k in ((p.codes, N, K), (p.codes_t, K, N)):
+        t = ops_untile(c, up(n, 256), up(k, 128))
+        assert not t[:, k:].any() and not t[n:].any()
 
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------

@@ -26,7 +26,7 @@ GATED = dict(W2=P, sw2=P, C=None, H=P, sh=P)
 @pytest.mark.parametrize("kw", [
     dict(M=-1), dict(N=0), dict(K=0), dict(X=None), dict(X=P + 8), dict(sx=None), dict(sx=P + 2), dict(W=None), dict(W=P + 4), dict(sw=None),
     dict(sw=P + 1), dict(C=None), dict(ldc=63), dict(act=2), dict(act=6), dict(act=-1), dict(act=3, residual=P, ldr=64),
-    dict(residual=P, ldr=63), dict(x=P, ldxr=129), dict(H=P), dict(sh=P), dict(K=1 << 22),
+    dict(residual=P, ldr=63), dict(x=P, ldxr=129), dict(H=P), dict(sh=P), dict(K=(1 << 17) + 1),
     {**GATED, "C": P}, {**GATED, "sw2": None}, {**GATED, "W2": P + 8}, {**GATED, "H": None}, {**GATED, "H": P + 4}, {**GATED, "sh": None},
     {**GATED, "bias": P}, {**GATED, "act": 5}, {**GATED, "residual": P, "ldr": 64}])
 def test_gemm_fp8_refuses(kw):
