@@ -3,150 +3,383 @@
 //   forward    out[i][:] = scale * table[ids[i]][:] + pos[i mod pos_rows][:]
 //   gradient   grad[v][:] = scale * sum over { i : ids[i] = v } of dy[i][:]
 //
-// Both are bound by HBM.  The gradient adds in a fixed order (no atomics): positions are ranked by (id, position), a chunk of the sorted
-// list is summed by one group of lanes, and runs of one token that cross a chunk's edge leave partial rows that a second pass adds in order.
+// Both are bound by HBM.  The gradient adds in a fixed order (no atomics): positions are ranked by (id, position), one wave sums a chunk of
+// the sorted list, and runs of one token that cross a chunk's edge leave partial rows that a last launch adds in order.  Three
+// launches: zeros together with the ranking, chunk sums, joins (and one before them where the list is long).
 // An id outside the table reads as a row of NaN (a gather cannot raise on the device) and its gradient is dropped.
 #include "fp8.h"
 
 namespace {
 
-constexpr int EMB_CHUNK = 32;          // sorted positions summed by one group of lanes
+constexpr int CHUNK = 16;              // sorted positions summed by one wave: its 16 rows are in flight together
+constexpr int32_t NONE = 0x7fffffff;   // key of an id outside the table: behind all others
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int ids64, int64_t i) {
   return ids64 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
 }
+template <typename T, int VEC>
+__device__ __forceinline__ void load_cols(const T* p, float v[VEC]) {
+  if constexpr (VEC == 1) {
+    if constexpr (sizeof(T) == 2) v[0] = bf2f(*p);
+    else v[0] = *p;
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+      const float4 t = *(const float4*)(p + k);
+      v[k] = t.x; v[k + 1] = t.y; v[k + 2] = t.z; v[k + 3] = t.w;
+    }
+  } else if constexpr (VEC == 4) {
+    const u16x4 t = *(const u16x4*)p;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = bf2f(t[k]);
+  } else {
+    const u16x8 t = *(const u16x8*)p;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = bf2f(t[k]);
+  }
+}
 
-// VEC columns of one token per thread
+// ---- lookup: one wave per token, VEC columns per lane and turn -------------------------------------------------------------------------
 template <typename T, typename O, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n,
                                                         float scale, const float* pos, int64_t pos_rows, int64_t ldp, O* out) {
-  const int per = D / VEC;
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (u >= n * per) return;
-  const int64_t i = u / per;
-  const int c = (int)(u - i * per) * VEC;
+  const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= n) return;
   const int64_t id = id_at(ids, ids64, i);
   const bool ok = id >= 0 && id < V;
-  const T* row = table + (ok ? id : 0) * ldt + c;
-  const float* pr = pos ? pos + (i % pos_rows) * ldp + c : nullptr;
-  float v[VEC];
+  const T* row = table + (ok ? id : 0) * ldt;
+  const float* pr = pos ? pos + (i % pos_rows) * ldp : nullptr;
+  O* o = out + i * D;
+  for (int c = (threadIdx.x & 63) * VEC; c < D; c += 64 * VEC) {
+    float v[VEC], q[VEC];
+    load_cols<T, VEC>(row + c, v);
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    float t;
-    if constexpr (sizeof(T) == 2) t = bf2f(row[k]);
-    else t = row[k];
-    v[k] = ok ? fmaf(scale, t, pr ? pr[k] : 0.f) : __uint_as_float(0x7fc00000u);
-  }
-  O* o = out + i * D + c;
+    for (int k = 0; k < VEC; ++k) q[k] = 0.f;
+    if (pr) load_cols<float, VEC>(pr + c, q);
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    if constexpr (sizeof(O) == 2) o[k] = f2bf(v[k]);
-    else o[k] = v[k];
+    for (int k = 0; k < VEC; ++k) v[k] = ok ? fmaf(scale, v[k], q[k]) : __uint_as_float(0x7fc00000u);
+    if constexpr (VEC == 1) {
+      if constexpr (sizeof(O) == 2) o[c] = f2bf(v[0]);
+      else o[c] = v[0];
+    } else if constexpr (sizeof(O) == 2) {
+      *(uint4*)(o + c) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+    } else {
+      *(float4*)(o + c) = make_float4(v[0], v[1], v[2], v[3]);
+      *(float4*)(o + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
   }
 }
 
-// position of i in the list sorted by (id, i); ids outside the table sort behind all others
-__global__ __launch_bounds__(256) void rank_kernel(const void* ids, int ids64, int64_t n, int64_t V, int32_t* sid, int32_t* spos) {
-  __shared__ int32_t key[256];
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  auto key_of = [&](int64_t p) {
-    const int64_t id = id_at(ids, ids64, p);
-    return id >= 0 && id < V ? (int32_t)id : 0x7fffffff;
-  };
-  const int32_t mine = i < n ? key_of(i) : 0;
-  int64_t rank = 0;
-  for (int64_t j0 = 0; j0 < n; j0 += 256) {
+// ---- gradient: the order ---------------------------------------------------------------------------------------------------------------
+// A position's place in the list sorted by (id, position) is the number of keys below its own.  Up to DIRECT positions they are counted
+// one by one (quadratic, but without a launch of its own: 3 us alone at 1 token, 6 at 1232, 17 at 4928).  Longer lists are first sorted
+// in parts of 256; the other parts' counts are then binary searches (16384 positions: 58 us counted directly, 131072: 1180 us).
+constexpr int DIRECT = 4096, PART = 256;
+constexpr int TILE = 4096;             // keys in LDS at a time
+
+__device__ __forceinline__ uint32_t key_of(const void* ids, int ids64, int64_t V, int64_t p) {
+  const int64_t id = id_at(ids, ids64, p);
+  return (uint32_t)(id >= 0 && id < V ? (int32_t)id : NONE);
+}
+// how many of 64 keys in LDS are below lim
+__device__ __forceinline__ int below64(const uint32_t* key, uint32_t lim) {
+  int r = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint4 k = ((const uint4*)key)[e];
+    r += (k.x < lim) + (k.y < lim) + (k.z < lim) + (k.w < lim);
+  }
+  return r;
+}
+// the same for the 64 keys of a wave's own positions: equal keys of earlier lanes come first
+__device__ __forceinline__ int below_own(const uint32_t* key, uint32_t mine, int lane) {
+  int r = 0;
+#pragma unroll
+  for (int e = 0; e < 64; ++e) r += key[e] < mine + (e < lane ? 1u : 0u);
+  return r;
+}
+
+__global__ __launch_bounds__(PART) void part_sort_kernel(const void* ids, int ids64, int64_t n, int64_t V, uint32_t* pkey, int32_t* ppos) {
+  __shared__ __attribute__((aligned(16))) uint32_t key[PART];
+  const int64_t p0 = (int64_t)blockIdx.x * PART, p = p0 + threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t mine = p < n ? key_of(ids, ids64, V, p) : 0xffffffffu;   // (behind everything; counted nowhere)
+  key[threadIdx.x] = mine;
+  __syncthreads();
+  int r = below_own(key + wave * 64, mine, lane);
+  for (int q = 0; q < PART / 64; ++q)
+    if (q != wave) r += below64(key + q * 64, mine + (q < wave && p < n ? 1u : 0u));
+  if (p >= n) r = threadIdx.x;                                            // (the last part's tail keeps its place)
+  pkey[p0 + r] = mine;
+  ppos[p0 + r] = (int32_t)p;
+}
+
+// blocks below `rankers` place positions, the others write zeros (the bulk of the bytes, which hides the order)
+template <bool PARTS>
+__global__ __launch_bounds__(256) void order_kernel(const void* ids, int ids64, int64_t n, int64_t V, const uint32_t* pkey, const int32_t* ppos,
+                                                    int rankers, int32_t* sid, int32_t* spos, float* g, int64_t rows, int D, int64_t ldg) {
+  if ((int)blockIdx.x >= rankers) {
+    const int64_t first = ((int64_t)blockIdx.x - rankers) * 256 + threadIdx.x, step = ((int64_t)gridDim.x - rankers) * 256, total = rows * D;
+    if (ldg == D && ((uintptr_t)g & 15) == 0) {
+      for (int64_t u = first; u < total / 4; u += step) ((float4*)g)[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (first < total % 4) g[total / 4 * 4 + first] = 0.f;
+    } else {
+      for (int64_t u = first; u < total; u += step) g[u / D * ldg + u % D] = 0.f;
+    }
+    return;
+  }
+  __shared__ __attribute__((aligned(16))) uint32_t key[TILE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if constexpr (!PARTS) {                        // 64 positions per block, the list shared out over its waves
+    __shared__ int32_t part[4][64];
+    const int64_t i0 = (int64_t)blockIdx.x * 64, i = i0 + lane;
+    const uint32_t mine = i < n ? key_of(ids, ids64, V, i) : 0;
+    const int groups = (int)((n + 63) >> 6);     // (n <= DIRECT = TILE: one tile)
+    for (int p = threadIdx.x; p < groups * 64; p += 256) key[p] = p < n ? key_of(ids, ids64, V, p) : 0xffffffffu;
     __syncthreads();
-    key[threadIdx.x] = j0 + threadIdx.x < n ? key_of(j0 + threadIdx.x) : 0x7fffffff;
+    int r = 0;
+    for (int q = wave; q < groups; q += 4)
+      r += q * 64 != i0 ? below64(key + q * 64, mine + (q * 64 < i0 ? 1u : 0u)) : below_own(key + q * 64, mine, lane);
+    part[wave][lane] = r;
     __syncthreads();
-    const int lim = (int)(n - j0 < 256 ? n - j0 : 256);
-    for (int j = 0; j < lim; ++j) rank += key[j] < mine || (key[j] == mine && j0 + j < i);
-  }
-  if (i < n) {
-    sid[rank] = mine;
-    spos[rank] = (int32_t)i;
-  }
-}
-
-__global__ __launch_bounds__(256) void fill_rows_kernel(float* g, int64_t V, int D, int64_t ldg) {
-  const int64_t total = V * D;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) g[u / D * ldg + u % D] = 0.f;
-}
-
-// one chunk of the sorted list, one column per thread.  part[c][0]: the run that came in over the chunk's left edge (the whole chunk, if it
-// also leaves over the right one); part[c][1]: the run that begins here and leaves over the right edge
-template <typename T>
-__global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy, const int32_t* sid, const int32_t* spos, int64_t n, int D,
-                                                      float scale, int accumulate, float* g, int64_t ldg, float* part) {
-  const int64_t p0 = (int64_t)blockIdx.x * EMB_CHUNK, p1 = p0 + EMB_CHUNK < n ? p0 + EMB_CHUNK : n;
-  const int col = blockIdx.y * 256 + threadIdx.x;
-  if (col >= D) return;
-  const int32_t before = p0 > 0 ? sid[p0 - 1] : -1, after = p1 < n ? sid[p1] : -1;
-  float sum = 0.f;
-  for (int64_t p = p0; p < p1; ++p) {
-    const int32_t id = sid[p];
-    const T* row = dy + (int64_t)spos[p] * lddy + col;
-    if constexpr (sizeof(T) == 2) sum += bf2f(*row);
-    else sum += *row;
-    const int32_t next = p + 1 < p1 ? sid[p + 1] : -2;
-    if (next == id) continue;
-    if (id != 0x7fffffff) {
-      if (id == before) part[((int64_t)blockIdx.x * 2) * D + col] = sum;
-      else if (next == -2 && id == after) part[((int64_t)blockIdx.x * 2 + 1) * D + col] = sum;
-      else {
-        float* o = g + (int64_t)id * ldg + col;
-        *o = accumulate ? fmaf(scale, sum, *o) : scale * sum;
+    if (wave == 0 && i < n) {
+      const int at = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+      sid[at] = (int32_t)mine;
+      spos[at] = (int32_t)i;
+    }
+  } else {                                       // one sorted part per block
+    const int64_t p = (int64_t)blockIdx.x * PART + threadIdx.x;
+    const uint32_t mine = pkey[p];
+    const int32_t pos = ppos[p];
+    const int parts = (int)((n + PART - 1) / PART);
+    int64_t at = threadIdx.x;
+    for (int c0 = 0; c0 < parts; c0 += TILE / PART) {
+      const int here = parts - c0 < TILE / PART ? parts - c0 : TILE / PART;
+      __syncthreads();
+      for (int q = threadIdx.x; q < here * PART; q += 256) key[q] = pkey[(int64_t)c0 * PART + q];
+      __syncthreads();
+#pragma unroll 4
+      for (int c = 0; c < here; ++c) {
+        const uint32_t lim = mine + (c0 + c < (int)blockIdx.x ? 1u : 0u);   // equal keys of earlier parts come first
+        const uint32_t* k = key + c * PART;
+        int lo = 0;
+#pragma unroll
+        for (int step = PART / 2; step > 0; step >>= 1) lo += k[lo + step - 1] < lim ? step : 0;
+        lo += k[lo] < lim;
+        at += c0 + c == (int)blockIdx.x ? 0 : lo;
       }
     }
-    sum = 0.f;
+    if (pos < n) {
+      sid[at] = (int32_t)mine;
+      spos[at] = pos;
+    }
   }
 }
 
-// runs that cross chunk edges: the block of the chunk where a run begins adds its partial rows in order
-__global__ __launch_bounds__(256) void run_join_kernel(const int32_t* sid, int64_t n, int D, float scale, int accumulate, float* g, int64_t ldg,
-                                                       const float* part) {
-  const int64_t c = blockIdx.x, p0 = c * EMB_CHUNK, p1 = p0 + EMB_CHUNK;
-  const int col = blockIdx.y * 256 + threadIdx.x;
-  if (col >= D || p1 >= n) return;
-  const int32_t id = sid[p1 - 1];
-  if (id == 0x7fffffff || sid[p1] != id || (p0 > 0 && sid[p0 - 1] == id)) return;
-  float sum = part[(c * 2 + 1) * D + col];
-  for (int64_t k = c + 1; k * EMB_CHUNK < n && sid[k * EMB_CHUNK] == id; ++k) sum += part[(k * 2) * D + col];
-  float* o = g + (int64_t)id * ldg + col;
-  *o = accumulate ? fmaf(scale, sum, *o) : scale * sum;
+template <int VEC>
+__device__ __forceinline__ void put_row(float* o, const float v[VEC], float scale, int accumulate) {
+  if constexpr (VEC == 1) {
+    *o = accumulate ? fmaf(scale, v[0], *o) : scale * v[0];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+      float4 t = make_float4(scale * v[k], scale * v[k + 1], scale * v[k + 2], scale * v[k + 3]);
+      if (accumulate) {
+        const float4 b = *(const float4*)(o + k);
+        t = make_float4(fmaf(scale, v[k], b.x), fmaf(scale, v[k + 1], b.y), fmaf(scale, v[k + 2], b.z), fmaf(scale, v[k + 3], b.w));
+      }
+      *(float4*)(o + k) = t;
+    }
+  }
 }
+
+// ---- second launch: one wave per chunk of the sorted list and 64 VEC columns -------------------------------------------------------------
+// part[c][0]: the run that came in over the chunk's left edge (the whole chunk, if it also leaves over the right one); part[c][1]: the run
+// that begins here and leaves over the right edge
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy, const int32_t* sid, const int32_t* spos, int64_t n, int D,
+                                                      int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part) {
+  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t c = unit / col_groups, p0 = c * CHUNK;
+  const int col = ((int)(unit - c * col_groups) * 64 + (threadIdx.x & 63)) * VEC;
+  if (p0 >= n || col >= D) return;
+  const int count = (int)(p0 + CHUNK < n ? CHUNK : n - p0);
+  const int32_t before = p0 > 0 ? sid[p0 - 1] : -1, after = p0 + CHUNK < n ? sid[p0 + CHUNK] : -1;
+  float v[CHUNK][VEC];
+  int32_t id[CHUNK];
+#pragma unroll
+  for (int q = 0; q < CHUNK; ++q) {
+    const int64_t p = p0 + (q < count ? q : count - 1);
+    id[q] = sid[p];
+    load_cols<T, VEC>(dy + (int64_t)spos[p] * lddy + col, v[q]);
+  }
+  float sum[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
+#pragma unroll
+  for (int q = 0; q < CHUNK; ++q) {
+    const bool here = q < count, last = q + 1 == count, ends = here && (last || id[q + 1 < CHUNK ? q + 1 : q] != id[q]);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum[k] = here ? sum[k] + v[q][k] : sum[k];
+    if (ends) {
+      if (id[q] != NONE) {
+        if (id[q] == before) put_row<VEC>(part + (c * 2) * D + col, sum, 1.f, 0);
+        else if (last && id[q] == after) put_row<VEC>(part + (c * 2 + 1) * D + col, sum, 1.f, 0);
+        else put_row<VEC>(g + (int64_t)id[q] * ldg + col, sum, scale, accumulate);
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
+    }
+  }
+}
+
+// ---- third launch: runs that cross chunk edges --------------------------------------------------------------------------------------------
+// A workgroup looks after the runs that begin in 16 chunks, for 64 VEC columns.  Runs over at most SHORT further chunks go to one wave
+// each; longer ones (padding) are shared out over the waves in contiguous parts that are added in order.
+constexpr int SHORT = 16, JOINERS = 16;
+template <int VEC>
+__global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* sid, int64_t n, int D, float scale, int accumulate, float* g,
+                                                                int64_t ldg, const float* part) {
+  __shared__ float share[JOINERS][64 * VEC];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = (blockIdx.y * 64 + lane) * VEC;
+  const int64_t chunks = (n + CHUNK - 1) / CHUNK, c = (int64_t)blockIdx.x * JOINERS + lane, p1 = (c + 1) * CHUNK;
+  bool mine = false, far = false;
+  if (lane < JOINERS && p1 < n) {
+    const int32_t id = sid[p1 - 1];
+    mine = id != NONE && sid[p1] == id && (c == 0 || sid[c * CHUNK - 1] != id);
+    far = mine && (c + 1 + SHORT) < chunks && sid[(c + 1 + SHORT) * CHUNK] == id;
+  }
+  uint64_t todo = __ballot(mine), longs = __ballot(far);
+  auto add_rows = [&](int64_t from, int64_t to, float s[VEC]) {        // part[k][0], from <= k < to
+    for (int64_t k = from; k < to; k += 16) {
+      float v[16][VEC];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) load_cols<float, VEC>(part + ((k + q < to ? k + q : to - 1) * 2) * D + col, v[q]);
+#pragma unroll
+      for (int q = 0; q < 16; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] = k + q < to ? s[e] + v[q][e] : s[e];
+    }
+  };
+  auto end_of = [&](int64_t first, int32_t id) {                       // the first chunk from `first` on that does not begin with id
+    for (int64_t step = 64; ; step = 1) {                              // by 64 at a time, then one by one
+      while (true) {
+        const int64_t k = first + (int64_t)lane * step;
+        const uint64_t no = __ballot(!(k < chunks && sid[k * CHUNK] == id));
+        if (no) {
+          const int b = __ffsll((long long)no) - 1;
+          if (step == 1) return first + b;
+          first += b ? (b - 1) * step + 1 : 0;
+          break;
+        }
+        first += 64 * step;
+      }
+    }
+  };
+  uint64_t near = todo & ~longs;
+  for (int turn = 0; near; ++turn) {
+    const int b = __ffsll((long long)near) - 1;
+    near &= near - 1;
+    if (turn % JOINERS != wave) continue;
+    const int64_t k = (int64_t)blockIdx.x * JOINERS + b;
+    const int32_t id = sid[(k + 1) * CHUNK - 1];
+    const int64_t end = end_of(k + 1, id);
+    if (col < D) {
+      float s[VEC];
+      load_cols<float, VEC>(part + (k * 2 + 1) * D + col, s);
+      add_rows(k + 1, end, s);
+      put_row<VEC>(g + (int64_t)id * ldg + col, s, scale, accumulate);
+    }
+  }
+  while (longs) {
+    const int b = __ffsll((long long)longs) - 1;
+    longs &= longs - 1;
+    const int64_t k = (int64_t)blockIdx.x * JOINERS + b;
+    const int32_t id = sid[(k + 1) * CHUNK - 1];
+    const int64_t end = end_of(k + 1, id), each = (end - (k + 1) + JOINERS - 1) / JOINERS;
+    const int64_t from = k + 1 + wave * each, to = from + each < end ? from + each : end;
+    float s[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s[e] = 0.f;
+    if (col < D) {
+      if (wave == 0) load_cols<float, VEC>(part + (k * 2 + 1) * D + col, s);
+      add_rows(from, to, s);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) share[wave][lane * VEC + e] = s[e];
+    __syncthreads();
+    if (wave == 0 && col < D) {
+      for (int q = 1; q < JOINERS; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += share[q][lane * VEC + e];
+      put_row<VEC>(g + (int64_t)id * ldg + col, s, scale, accumulate);
+    }
+    __syncthreads();
+  }
+}
+
+bool aligned16(const void* p, int64_t ld_bytes) { return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0; }
 
 }  // namespace
 
 int launch_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n, float scale,
                      const float* pos, int64_t pos_rows, int64_t ldp, void* out, int out_f32, hipStream_t st) {
   if (n == 0) return 0;
-  const int64_t blocks = (n * D + 255) / 256;
+  const int64_t blocks = (n + 3) / 4;
   FDMI_CHECK(blocks < (1ll << 31), "embed_fwd: too many tokens");
-#define EMB_FWD(T, O) hipLaunchKernelGGL((embed_fwd_kernel<T, O, 1>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)table, V, D, ldt, ids, \
-                                         ids64, n, scale, pos, pos_rows, ldp, (O*)out)
-  if (table_f32) { if (out_f32) EMB_FWD(float, float); else EMB_FWD(float, bf16_t); }
-  else { if (out_f32) EMB_FWD(bf16_t, float); else EMB_FWD(bf16_t, bf16_t); }
+  const bool vec = D % 8 == 0 && aligned16(table, ldt * (table_f32 ? 4 : 2)) && (!pos || aligned16(pos, ldp * 4)) && aligned16(out, 0);
+#define EMB_FWD(T, O, VEC) hipLaunchKernelGGL((embed_fwd_kernel<T, O, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)table, V, D, ldt, \
+                                              ids, ids64, n, scale, pos, pos_rows, ldp, (O*)out)
+  if (table_f32) { if (out_f32) { if (vec) EMB_FWD(float, float, 8); else EMB_FWD(float, float, 1); }
+                   else { if (vec) EMB_FWD(float, bf16_t, 8); else EMB_FWD(float, bf16_t, 1); } }
+  else { if (out_f32) { if (vec) EMB_FWD(bf16_t, float, 8); else EMB_FWD(bf16_t, float, 1); }
+         else { if (vec) EMB_FWD(bf16_t, bf16_t, 8); else EMB_FWD(bf16_t, bf16_t, 1); } }
 #undef EMB_FWD
   FDMI_HIP(hipGetLastError());
   return 0;
 }
 
-int64_t embed_bwd_ws_bytes(int64_t n, int D) {
-  return (n * 2 * 4 + 255) / 256 * 256 + (n + EMB_CHUNK - 1) / EMB_CHUNK * 2 * (int64_t)D * 4;
-}
+// scratch: the sorted list's keys and positions, those of the sorted parts, and two partial rows per chunk
+static int64_t list_bytes(int64_t n) { return ((n > DIRECT ? n + (n + PART - 1) / PART * PART : n) * 2 * 4 + 255) / 256 * 256; }
+int64_t embed_bwd_ws_bytes(int64_t n, int D) { return list_bytes(n) + (n + CHUNK - 1) / CHUNK * 2 * (int64_t)D * 4; }
 int launch_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
                      int accumulate, float* grad, int64_t ldg, void* ws, hipStream_t st) {
-  if (!accumulate) hipLaunchKernelGGL(fill_rows_kernel, dim3(4096), dim3(256), 0, st, grad, V, D, ldg);
+  const bool parts = n > DIRECT;
+  const int np = cdiv(n, PART);
+  int32_t* sid = (int32_t*)ws;
+  int32_t* spos = sid + n;
+  uint32_t* pkey = (uint32_t*)(spos + n);
+  int32_t* ppos = (int32_t*)pkey + (int64_t)np * PART;
+  float* part = (float*)((char*)ws + list_bytes(n));
+  const int rankers = parts ? np : cdiv(n, 64);
+  const int64_t fills = accumulate ? 0 : ((int64_t)V * D + 4095) / 4096;
+  const int fillers = (int)(fills < 2048 ? fills : 2048);
+  if (parts) {
+    hipLaunchKernelGGL(part_sort_kernel, dim3(np), dim3(PART), 0, st, ids, ids64, n, V, pkey, ppos);
+    hipLaunchKernelGGL(order_kernel<true>, dim3(rankers + fillers), dim3(256), 0, st, ids, ids64, n, V, pkey, ppos, rankers, sid, spos, grad, V,
+                       D, ldg);
+  } else if (rankers + fillers) {
+    hipLaunchKernelGGL(order_kernel<false>, dim3(rankers + fillers), dim3(256), 0, st, ids, ids64, n, V, nullptr, nullptr, rankers, sid, spos,
+                       grad, V, D, ldg);
+  }
   if (n > 0) {
-    int32_t* sid = (int32_t*)ws;
-    int32_t* spos = sid + n;
-    float* part = (float*)((char*)ws + (n * 2 * 4 + 255) / 256 * 256);
-    const dim3 grid(cdiv(n, EMB_CHUNK), cdiv(D, 256));
-    hipLaunchKernelGGL(rank_kernel, dim3(cdiv(n, 256)), dim3(256), 0, st, ids, ids64, n, V, sid, spos);
-    if (dy_f32) hipLaunchKernelGGL(run_sum_kernel<float>, grid, dim3(256), 0, st, (const float*)dy, lddy, sid, spos, n, D, scale, accumulate, grad, ldg, part);
-    else hipLaunchKernelGGL(run_sum_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)dy, lddy, sid, spos, n, D, scale, accumulate, grad, ldg, part);
-    hipLaunchKernelGGL(run_join_kernel, grid, dim3(256), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
+    const bool vec = D % 4 == 0 && aligned16(dy, lddy * 4) && (dy_f32 || lddy % 4 == 0) && aligned16(grad, ldg * 4);
+    const bool vec8 = vec && !dy_f32 && D % 8 == 0 && lddy % 8 == 0;                       // (16 bytes of a bf16 row per lane)
+    const int groups = cdiv(D, vec8 ? 512 : vec ? 256 : 64);
+    const int64_t chunks = (n + CHUNK - 1) / CHUNK, blocks = (chunks * groups + 3) / 4;
+    FDMI_CHECK(blocks < (1ll << 31), "embed_bwd: too many tokens");
+    const dim3 join((unsigned)((chunks + JOINERS - 1) / JOINERS), cdiv(D, vec ? 256 : 64));
+#define EMB_SUM(T, VEC) hipLaunchKernelGGL((run_sum_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)dy, lddy, sid, spos, n, D, \
+                                           groups, scale, accumulate, grad, ldg, part)
+    if (vec) {
+      if (dy_f32) EMB_SUM(float, 4); else if (vec8) EMB_SUM(bf16_t, 8); else EMB_SUM(bf16_t, 4);
+      hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
+    } else {
+      if (dy_f32) EMB_SUM(float, 1); else EMB_SUM(bf16_t, 1);
+      hipLaunchKernelGGL(run_join_kernel<1>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
+    }
+#undef EMB_SUM
   }
   FDMI_HIP(hipGetLastError());
   return 0;

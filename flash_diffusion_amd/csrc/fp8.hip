@@ -15,6 +15,7 @@
 // zeros to 256 rows, so a tile's loads need no bounds there.
 #include "fp8.h"
 #include "gemm.h"
+#include <atomic>
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -566,11 +567,22 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
   dma_wait<0>();                                  // no transfer may be on its way when the workgroup's LDS is released
 }
 
+// the kernel's allowance of dynamic LDS, asked for once per device (`done`: one bit for each)
+int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  FDMI_HIP(hipGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return 0;
+  FDMI_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return 0;
+}
+
 template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE, bool VEC>
 int launch_tile(const Fp8GemmArgs& a, hipStream_t st) {
   constexpr int most = fp8_smem(BM, BN, WM, WN, GATED, VEC, SEG);
   static_assert(most <= 160 * 1024, "LDS");
-  FDMI_HIP(hipFuncSetAttribute((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, most));
+  static std::atomic<uint64_t> allowed;
+  if (const int rc = allow_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE, VEC>, most, allowed)) return rc;
   const int smem = fp8_smem(BM, BN, WM, WN, GATED, VEC, a.Kb);
   const int64_t tilesM = ((int64_t)a.M + BM - 1) / BM, tilesN = ((int64_t)a.N * (GATED ? 2 : 1) + BN - 1) / BN;
   FDMI_CHECK(tilesM * tilesN < (1ll << 30), "gemm_fp8: too many tiles");
@@ -678,7 +690,8 @@ template <int MT, int NT, bool WIDE>
 int launch_stream(const Fp8GemmArgs& a, hipStream_t st) {
   constexpr int smem = fp8_stream_smem(MT, NT);
   static_assert(smem <= 160 * 1024, "LDS");
-  FDMI_HIP(hipFuncSetAttribute((const void*)fp8_stream_kernel<MT, NT, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> allowed;
+  if (const int rc = allow_lds((const void*)fp8_stream_kernel<MT, NT, WIDE>, smem, allowed)) return rc;
   const dim3 grid(cdiv(a.N, NT * 16), cdiv(a.M, MT * 16));
   hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE>), grid, dim3(512), smem, st, a);
   FDMI_HIP(hipGetLastError());

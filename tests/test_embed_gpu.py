@@ -75,7 +75,8 @@ def _ids_of(kind, n, V, seed):
 
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("kind", ["one", "all", "runs", "padded"])
-@pytest.mark.parametrize("n,V,D", [(1, 1, 1), (31, 7, 3), (32, 50, 64), (33, 50, 65), (64, 300, 130), (257, 100, 257), (1232, 2000, 96), (5000, 700, 40)])
+@pytest.mark.parametrize("n,V,D", [(1, 1, 1), (31, 7, 3), (32, 50, 64), (33, 50, 65), (64, 300, 130), (257, 100, 257), (1232, 2000, 96), (4096, 900, 12),
+                                   (4097, 900, 12), (5000, 700, 40), (20000, 3000, 5)])
 def test_gradient(n, V, D, kind, dt):
     ops = _ops()
     ids = _ids_of(kind, n, V, n + V)
