@@ -156,6 +156,7 @@ _SIGS = {
     "fdmi_quant_fp8": (i32, [vp, i32, i64, vp, f32, vp, vp, i64, i32, vp]),
     "fdmi_pack_fp8": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp]),
     "fdmi_gemm_fp8": (i32, [C.POINTER(Fp8Desc), vp]),
+    "fdmi_fp8_scratch_bytes": (i64, [i64, i32]),
     "fdmi_embed_fwd": (i32, [vp, i32, i64, i32, i64, vp, i32, i64, f32, vp, i64, i64, vp, i32, vp]),
     "fdmi_embed_bwd_ws_bytes": (i64, [i64, i32]),
     "fdmi_embed_bwd": (i32, [vp, i32, i64, vp, i32, i64, i64, i32, f32, i32, vp, i64, vp, vp]),

@@ -473,7 +473,8 @@ int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* cod
 int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
   FDMI_CHECK(d && d->M >= 0 && d->N >= 1 && d->K >= 1, "gemm_fp8: need M >= 0, N >= 1, K >= 1");
   if (d->M == 0) return 0;
-  FDMI_CHECK(fp8_ok(d->X, d->sx, d->K) && fp8_ok(d->W, d->sw, d->K), "gemm_fp8: codes are 16-byte, scales 4-byte aligned, K <= 131072");
+  const bool fused = d->x && !d->W2 && fp8_fused(d->M, d->K);
+  FDMI_CHECK((fused || fp8_ok(d->X, d->sx, d->K)) && fp8_ok(d->W, d->sw, d->K), "gemm_fp8: codes are 16-byte, scales 4-byte aligned, K <= 131072");
   FDMI_CHECK(!d->x || d->ldxr >= d->K, "gemm_fp8: x rows shorter than K");
   Fp8GemmArgs a;
   a.X = (const uint8_t*)d->X; a.sx = (const uint8_t*)d->sx;
@@ -494,11 +495,18 @@ int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
     FDMI_CHECK(d->act == ACT_NONE || !d->residual, "gemm_fp8: an activation and a residual exclude each other");
     a.bias = d->bias; a.residual = d->residual; a.ldr = d->ldr; a.C = d->C; a.ldc = d->ldc; a.out_f32 = d->out_f32; a.act = d->act;
   }
-  if (d->x) {
+  if (fused) {
+    const int es = d->x_f32 ? 4 : 2;
+    a.x = d->x; a.ldxr = d->ldxr; a.x_f32 = d->x_f32; a.K = d->K;
+    a.xvec = ((uintptr_t)d->x & 15) == 0 && d->ldxr * es % 16 == 0;
+  } else if (d->x) {
     const int rc = launch_quant_fp8(d->x, d->x_f32, d->ldxr, nullptr, 0.f, (uint8_t*)d->X, (uint8_t*)d->sx, d->M, d->K, (hipStream_t)stream);
     if (rc) return rc;
   }
   return launch_gemm_fp8(a, (hipStream_t)stream);
+}
+int64_t fdmi_fp8_scratch_bytes(int64_t M, int K) {
+  return M < 1 || K < 1 || fp8_fused(M, K) ? 0 : (M + 15) / 16 * 16 * cdiv(K, 128) * 129;
 }
 int fdmi_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n, float scale,
                    const float* pos, int64_t pos_rows, int64_t ldp, void* out, int out_f32, void* stream) {

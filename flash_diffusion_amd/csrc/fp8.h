@@ -9,12 +9,14 @@ struct Fp8GemmArgs {
   const uint8_t* W = nullptr; const uint8_t* sw = nullptr;
   const uint8_t* W2 = nullptr; const uint8_t* sw2 = nullptr;
   int M = 0, N = 0, Kb = 0;
+  const void* x = nullptr; int64_t ldxr = 0; int x_f32 = 0, K = 0; bool xvec = false;   // unquantised rows in X's place (fp8_fused problems)
   const float* bias = nullptr;
   const void* residual = nullptr; int64_t ldr = 0;             // of C's type
   void* C = nullptr; int64_t ldc = 0; int out_f32 = 0;
   int act = 0;
   uint8_t* H = nullptr; uint8_t* sh = nullptr;
 };
+bool fp8_fused(int64_t M, int K);
 int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st);
 int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, uint8_t* q, uint8_t* s, int64_t M, int K,
                      hipStream_t st);

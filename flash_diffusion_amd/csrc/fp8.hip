@@ -16,6 +16,7 @@
 #include "fp8.h"
 #include "gemm.h"
 #include <atomic>
+#include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -73,9 +74,37 @@ __device__ __forceinline__ void load16(const T* p, int k, int K, bool vec, float
   load8(p, k, K, vec, v);
   load8(p, k + 8, K, vec, v + 8);
 }
+// a block of 128 held by eight lanes, 16 values each, that differ in the lane bits o0, o1, o2: its scale byte.  Infinities are rare: they are
+// seen in the maximum (fmax drops a NaN), only then replaced by NaN and the maximum taken again over the finite values; the values
+// left are within +-448 after scaling, or NaN, which the conversion keeps
+__device__ __forceinline__ int block_scale(float v[16], int o0, int o1, int o2) {
+  float a = fabsf(v[0]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) a = fmaxf(a, fabsf(v[i]));
+  auto over = [&](float t) {
+    t = fmaxf(t, __shfl_xor(t, o0, 64));
+    t = fmaxf(t, __shfl_xor(t, o1, 64));
+    return fmaxf(t, __shfl_xor(t, o2, 64));
+  };
+  a = over(a);
+  if (a > 3.402823466e38f) {
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (fabsf(v[i]) > 3.402823466e38f) v[i] = __uint_as_float(0x7fc00000u);
+      a = fmaxf(a, fabsf(v[i]));
+    }
+    a = over(a);
+  }
+  return scale_byte(a != a ? 0.f : a);             // (a block of nothing but NaN)
+}
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
 __device__ __forceinline__ uint4 codes16(const float v[16], float up) {
-  return make_uint4(codes4(v[0], v[1], v[2], v[3], up), codes4(v[4], v[5], v[6], v[7], up), codes4(v[8], v[9], v[10], v[11], up),
-                    codes4(v[12], v[13], v[14], v[15], up));
+  return make_uint4(pack4(v[0] * up, v[1] * up, v[2] * up, v[3] * up), pack4(v[4] * up, v[5] * up, v[6] * up, v[7] * up),
+                    pack4(v[8] * up, v[9] * up, v[10] * up, v[11] * up), pack4(v[12] * up, v[13] * up, v[14] * up, v[15] * up));
 }
 
 // ---- rows of activations -------------------------------------------------------------------------------------------------------------
@@ -90,6 +119,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, int64_t ldx
   if constexpr (NORM) {
     const T* row = x + (m0 + wave < M ? m0 + wave : M - 1) * ldx;
     float ss = 0.f, v[8];
+#pragma unroll 4
     for (int k = lane * 8; k < K; k += 512) {
       load8(row, k, K, vec, v);
 #pragma unroll
@@ -102,26 +132,29 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, int64_t ldx
   const int r = lane & 3, c = lane >> 2;
   const int64_t m = m0 + r;
   const T* row = x + (m < M ? m : M - 1) * ldx;
-  const int first = NORM ? wave * 256 : (blockIdx.y * 4 + wave) * 256, step = NORM ? 1024 : Kb * 128;
-  for (int k0 = first; k0 < Kb * 128; k0 += step) {
-    const int k = k0 + c * 16;
-    float v[16], g[16];
-    load16(row, k, m < M ? K : 0, vec, v);
+  const int width = Kb * 128, cols = m < M ? K : 0;
+  // two pieces of 256 columns in flight per wave: a grid of four rows x 2048 columns, or, behind a norm, all columns of the four rows
+  const int first = NORM ? wave * 256 : blockIdx.y * 2048 + wave * 256, stop = NORM || first >= width ? width : first + 1;
+  for (int k0 = first; k0 < stop; k0 += 2048) {
+    float v[2][16], g[2][16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load16(row, k0 + h * 1024 + c * 16, cols, vec, v[h]);
     if constexpr (NORM) {
-      load16(w, k, K, wvec, g);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) load16(w, k0 + h * 1024 + c * 16, K, wvec, g[h]);
       const float rr = rs[r];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = v[i] * rr * g[i];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[h][i] = v[h][i] * rr * g[h][i];
     }
-    float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) a = fmaxf(a, finite_abs(v[i]));
-#pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) a = fmaxf(a, __shfl_xor(a, o, 64));   // the eight chunks of a block of 128
-    const int byte = scale_byte(a);
-    if (k < Kb * 128) {
-      *(uint4*)(q + ((m >> 4) * Kb * 2 + (k >> 6)) * 1024 + (c & 3) * 256 + (m & 15) * 16) = codes16(v, scale_up(byte));
-      if ((c & 7) == 0) s[(k >> 7) * Mp + m] = (uint8_t)byte;
+    for (int h = 0; h < 2; ++h) {
+      const int k = k0 + h * 1024 + c * 16, byte = block_scale(v[h], 4, 8, 16);
+      if (k < width) {
+        *(uint4*)(q + ((m >> 4) * Kb * 2 + (k >> 6)) * 1024 + (c & 3) * 256 + (m & 15) * 16) = codes16(v[h], scale_up(byte));
+        if ((c & 7) == 0) s[(k >> 7) * Mp + m] = (uint8_t)byte;
+      }
     }
   }
 }
@@ -602,9 +635,10 @@ int launch_tile(const Fp8GemmArgs& a, hipStream_t st) {
 // out the contraction (block kb goes to wave kb % 8), fetch whole tiles straight into matrix fragments -- a lane's two 16-byte reads of
 // a 16 x 128 pair of tiles are v_mfma_scale_f32_16x16x128's operand -- DEPTH blocks at a time, and join their sums through LDS in the
 // order of the waves.  No split over workgroups: N / 16 of them fill the chip from N = 4096 on, and smaller weights sit in L2.
+constexpr int FUSE = 1 << 16;            // bytes of codes that a workgroup quantises for itself
 constexpr int fp8_stream_smem(int MT, int NT) { return 8 * MT * 16 * (NT * 16 + 4) * 4; }
 
-template <int MT, int NT, bool WIDE>
+template <int MT, int NT, bool WIDE, typename RAW>
 __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int DEPTH = MT * 2 + NT * 2 <= 4 ? 4 : MT * 2 + NT * 2 <= 8 ? 2 : 1, LD = NT * 16 + 4;
@@ -612,6 +646,8 @@ __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
   const int64_t panel = (int64_t)a.Kb * 2048;
   const int Mt = (a.M + 15) >> 4, mt0 = blockIdx.y * MT, nt0 = blockIdx.x * NT;
   const int64_t Mp = (int64_t)Mt * 16, Ng = (int64_t)((a.N + 255) >> 8) * 8;
+  constexpr bool FUSED = !std::is_void<RAW>::value;
+  static_assert(!FUSED || MT == 1, "sixteen rows");
   const uint8_t* wp[NT];
   const uint8_t* xp[MT];
   const uint8_t* sxp[MT];
@@ -629,20 +665,49 @@ __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int k = 0; k < MT; ++k) acc[i][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int kb0 = wave; kb0 < a.Kb; kb0 += 8 * DEPTH) {
-    i32x8 w[DEPTH][NT], x[DEPTH][MT];
-    int sw[DEPTH], sx[DEPTH][MT];
+  i32x8 w[DEPTH][NT], x[DEPTH][MT];
+  int sw[DEPTH], sx[DEPTH][MT];
+  auto fetch_w = [&](int kb0) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const int kb = kb0 + 8 * d < a.Kb ? kb0 + 8 * d : kb0;
-      const int64_t o = (int64_t)kb * 2048;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) w[d][i] = join(*(const uint4*)(wp[i] + o), *(const uint4*)(wp[i] + o + 1024));
-#pragma unroll
-      for (int k = 0; k < MT; ++k) x[d][k] = join(*(const uint4*)(xp[k] + o), *(const uint4*)(xp[k] + o + 1024));
+      for (int i = 0; i < NT; ++i) w[d][i] = join(*(const uint4*)(wp[i] + (int64_t)kb * 2048), *(const uint4*)(wp[i] + (int64_t)kb * 2048 + 1024));
       sw[d] = swp[kb * Ng];                                            // (16 NT rows lie in one group of 32)
+    }
+  };
+  if constexpr (FUSED) {
+    // the rows come unquantised: every workgroup quantises all of them into LDS, [chunk of 16 columns][row][16 bytes] and scales behind
+    // (at most FUSE bytes of codes; one launch instead of two), while its first tiles of W are on their way
+    if (wave < a.Kb) fetch_w(wave);
+    const int per = a.Kb * 8;
+    uint8_t* sq = (uint8_t*)smem + a.M * per * 16;
+    for (int u = threadIdx.x; u < a.M * per; u += 512) {
+      const int m = u / per, c = u - m * per;
+      float v[16];
+      load16((const RAW*)a.x + (int64_t)m * a.ldxr, c * 16, a.K, a.xvec, v);
+      const int byte = block_scale(v, 1, 2, 4);
+      *(uint4*)(smem + (c * a.M + m) * 16) = codes16(v, scale_up(byte));
+      if ((c & 7) == 0) sq[(c >> 3) * a.M + m] = (uint8_t)byte;
+    }
+    __syncthreads();
+  }
+  for (int kb0 = wave; kb0 < a.Kb; kb0 += 8 * DEPTH) {
+    if (!FUSED || kb0 != wave) fetch_w(kb0);
 #pragma unroll
-      for (int k = 0; k < MT; ++k) sx[d][k] = sxp[k][kb * Mp];
+    for (int d = 0; d < DEPTH; ++d) {
+      const int kb = kb0 + 8 * d < a.Kb ? kb0 + 8 * d : kb0;
+      if constexpr (FUSED) {
+        const int m = (lane & 15) < a.M ? lane & 15 : a.M - 1, c = kb * 8 + (lane >> 4);
+        x[d][0] = join(*(const uint4*)(smem + (c * a.M + m) * 16), *(const uint4*)(smem + ((c + 4) * a.M + m) * 16));
+        sx[d][0] = ((const uint8_t*)smem)[a.M * a.Kb * 128 + kb * a.M + m];
+      } else {
+        const int64_t o = (int64_t)kb * 2048;
+#pragma unroll
+        for (int k = 0; k < MT; ++k) x[d][k] = join(*(const uint4*)(xp[k] + o), *(const uint4*)(xp[k] + o + 1024));
+#pragma unroll
+        for (int k = 0; k < MT; ++k) sx[d][k] = sxp[k][kb * Mp];
+      }
     }
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
@@ -671,6 +736,7 @@ __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
   }
   // lane l holds output row l & 15 and columns 4 (l >> 4) + 0 .. 3 of each fragment
   float* red = (float*)smem;
+  if constexpr (FUSED) __syncthreads();                                // (the codes lie there)
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -686,14 +752,15 @@ __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
   }
 }
 
-template <int MT, int NT, bool WIDE>
+template <int MT, int NT, bool WIDE, typename RAW>
 int launch_stream(const Fp8GemmArgs& a, hipStream_t st) {
-  constexpr int smem = fp8_stream_smem(MT, NT);
-  static_assert(smem <= 160 * 1024, "LDS");
+  constexpr int join = fp8_stream_smem(MT, NT), most = std::is_void<RAW>::value ? join : FUSE + FUSE / 128;
+  static_assert(join <= most && most <= 160 * 1024, "LDS");
   static std::atomic<uint64_t> allowed;
-  if (const int rc = allow_lds((const void*)fp8_stream_kernel<MT, NT, WIDE>, smem, allowed)) return rc;
+  if (const int rc = allow_lds((const void*)fp8_stream_kernel<MT, NT, WIDE, RAW>, most, allowed)) return rc;
+  const int codes = std::is_void<RAW>::value ? 0 : a.M * a.Kb * 129, smem = join > codes ? join : codes;
   const dim3 grid(cdiv(a.N, NT * 16), cdiv(a.M, MT * 16));
-  hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE>), grid, dim3(512), smem, st, a);
+  hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE, RAW>), grid, dim3(512), smem, st, a);
   FDMI_HIP(hipGetLastError());
   return 0;
 }
@@ -708,8 +775,8 @@ int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, f
   const bool vec = aligned(x, ldx * (x_f32 ? 4 : 2), 16), wvec = ((uintptr_t)norm % 16) == 0;
   const int Kb = cdiv(K, 128);
   const int64_t Mp = (M + 15) / 16 * 16, rows4 = (M + 3) / 4;
-  FDMI_CHECK(rows4 < (1ll << 31) && cdiv(Kb, 8) < 65536, "quant_fp8: too many rows or columns");
-  const dim3 grid((unsigned)rows4, norm ? 1 : cdiv(Kb, 8));
+  FDMI_CHECK(rows4 < (1ll << 31) && cdiv(Kb, 16) < 65536, "quant_fp8: too many rows or columns");
+  const dim3 grid((unsigned)rows4, norm ? 1 : cdiv(Kb, 16));
 #define FP8_QUANT(T, NORM) hipLaunchKernelGGL((quant_rows_kernel<T, NORM>), grid, dim3(256), 0, st, (const T*)x, ldx, norm, eps, q, s, M, Mp, K, Kb, vec, wvec)
   if (norm) { if (x_f32) FP8_QUANT(float, true); else FP8_QUANT(bf16_t, true); }
   else { if (x_f32) FP8_QUANT(float, false); else FP8_QUANT(bf16_t, false); }
@@ -744,8 +811,15 @@ double fp8_stream_cost(const Fp8GemmArgs& a, int rows) {   // `rows` rows of X a
   return 2.7 + (l2 > hbm ? l2 : hbm);
 }
 
+// whether a product of unquantised rows quantises them inside the streaming kernel
+bool fp8_fused(int64_t M, int K) { return M <= 16 && M * cdiv(K, 128) * 128 <= FUSE; }
+
 int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st) {
   if (a.M == 0) return 0;
+  if (a.x) {   // unquantised rows without scratch (fp8_fused)
+    if (a.x_f32) return a.out_f32 ? launch_stream<1, 1, true, float>(a, st) : launch_stream<1, 1, false, float>(a, st);
+    return a.out_f32 ? launch_stream<1, 1, true, bf16_t>(a, st) : launch_stream<1, 1, false, bf16_t>(a, st);
+  }
   if (a.H) return a.M <= 64 ? launch_tile<64, 256, 1, 4, true, false, true>(a, st) : launch_tile<128, 256, 2, 4, true, false, true>(a, st);
   const int es = a.out_f32 ? 4 : 2;
   const bool vec = a.N % 8 == 0 && aligned(a.C, a.ldc * es, 16) && (!a.residual || aligned(a.residual, a.ldr * es, 16)) && ((uintptr_t)a.bias & 15) == 0;
@@ -760,8 +834,8 @@ int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st) {
     if (best < 0 || c < least) { best = i; least = c; }
   }
   const double s16 = fp8_stream_cost(a, 16), s32 = fp8_stream_cost(a, 32);
-  if (s16 <= s32 && s16 < least) return a.out_f32 ? launch_stream<1, 1, true>(a, st) : launch_stream<1, 1, false>(a, st);
-  if (s32 < least) return a.out_f32 ? launch_stream<2, 2, true>(a, st) : launch_stream<2, 2, false>(a, st);
+  if (s16 <= s32 && s16 < least) return a.out_f32 ? launch_stream<1, 1, true, void>(a, st) : launch_stream<1, 1, false, void>(a, st);
+  if (s32 < least) return a.out_f32 ? launch_stream<2, 2, true, void>(a, st) : launch_stream<2, 2, false, void>(a, st);
 #define FP8_TILE(BM, BN, WM, WN, WIDE) (vec ? launch_tile<BM, BN, WM, WN, false, WIDE, true>(a, st) : launch_tile<BM, BN, WM, WN, false, WIDE, false>(a, st))
   switch (table[best].BM + table[best].BN) {
     case 128: return a.out_f32 ? FP8_TILE(64, 64, 2, 2, true) : FP8_TILE(64, 64, 2, 2, false);

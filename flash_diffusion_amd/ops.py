@@ -535,7 +535,7 @@ def rmsnorm_fp8(x, w, eps):
     return o
 
 
-def _fp8_rows_of(d, A, K, what):
+def _fp8_rows_of(d, A, K, what, gated=False):
     """fills the activation side of a descriptor from Fp8Rows or from [M, K] bf16 / f32 rows (quantised by the call itself); returns what has
     to stay alive until the launch"""
     if isinstance(A, Fp8Rows):
@@ -547,10 +547,13 @@ def _fp8_rows_of(d, A, K, what):
     M, cols = A.shape
     if cols != K:
         raise ValueError(f"{what} has {cols} columns, the weight contracts over {K}")
+    d.M, d.x, d.x_f32 = M, A.data_ptr(), A.dtype == F32
     n = _pad(M, 16) * (_pad(K, 128) // 128)
+    if not gated and not lib().fdmi_fp8_scratch_bytes(M, K):
+        return A
     scratch = torch.empty(n * 129, dtype=torch.uint8, device=A.device)
     p = scratch.data_ptr()
-    d.M, d.x, d.x_f32, d.X, d.sx = M, A.data_ptr(), A.dtype == F32, p, p + n * 128
+    d.X, d.sx = p, p + n * 128
     return scratch
 
 
@@ -600,7 +603,7 @@ def gated_fp8(A, W, W2):
     if (W.N, W.K) != (W2.N, W2.K):
         raise ValueError(f"the two weights differ in shape: {(W.N, W.K)} and {(W2.N, W2.K)}")
     d = Fp8Desc()
-    keep = _fp8_rows_of(d, A, W.K, "A")
+    keep = _fp8_rows_of(d, A, W.K, "A", gated=True)
     o = Fp8Rows(d.M, W.N, keep.device)
     d.N, d.K = W.N, W.K
     d.W, d.sw = _here(W.codes, "weight").data_ptr(), W.scales.data_ptr()

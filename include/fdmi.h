@@ -224,7 +224,8 @@ int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* cod
                   void* stream);
 /* C[M][N] = act(X W^T + bias) or X W^T + bias + residual, summed in fp32, rounded once to C's type (bf16, or fp32 when out_f32; the
  * residual has C's type).  X / sx: codes and scales -- or, when x is given, the unquantised activations x [M][K], and X / sx is scratch of
- * that size which may be written.  W2 given: the gated form; W and W2 are two weights of one shape and
+ * that size which may be written (not needed where fdmi_fp8_scratch_bytes says 0: a few rows, not gated, are quantised inside the
+ * product).  W2 given: the gated form; W and W2 are two weights of one shape and
  * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H, sh (M rows of N columns; the wi_0 / wi_1 pair of a gated feed-forward; no C,
  * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product.                                          */
 typedef struct fdmi_fp8_desc {
@@ -239,6 +240,7 @@ typedef struct fdmi_fp8_desc {
   void* H; void* sh;
 } fdmi_fp8_desc;
 int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream);
+int64_t fdmi_fp8_scratch_bytes(int64_t M, int K);   /* of codes and scales together: the scales lie behind R * Kb * 128 bytes of codes */
 
 /* ---------------- token-embedding lookup and its gradient (csrc/embed.hip) ----------------
  * out[i][:] = scale * table[ids[i]][:] + pos[i mod pos_rows][:]  (table fp32 or bf16 [V][D], pos fp32 or NULL, ids int32 or int64,

@@ -77,6 +77,7 @@ def test_all_256_codes_are_their_own_rounding_and_midpoints_go_to_even():
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_infinities_and_nan_become_nan_and_leave_the_scale_alone(dtype):
+    """(the product of three rows quantises them inside, that of forty does not)"""
     x = _rand(3, 256, dtype=dtype)
     x[0, 5], x[0, 6], x[1, 200] = float("inf"), float("nan"), float("-inf")
     x[2, :128] = float("nan")
@@ -85,8 +86,12 @@ def test_infinities_and_nan_become_nan_and_leave_the_scale_alone(dtype):
     got = _np(q.values(F32))
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~np.isnan(got)], want[~np.isnan(want)])
     w = _ops().pack_weight_fp8(_rand(70, 256, seed=3).cuda())
+    for rep in (1, 14):
+        y = _ops().gemm_fp8(x.cuda().repeat(rep, 1), w, out_f32=True)
+        assert bool(torch.isnan(y).all())                                   # every row holds one
+    x[1] = 1.0                                                              # ... and one that holds none is not touched
     y = _ops().gemm_fp8(x.cuda(), w, out_f32=True)
-    assert bool(torch.isnan(y).all())                                       # every row holds one
+    assert bool(torch.isfinite(y[1]).all()) and bool(torch.isnan(y[0]).all())
 
 
 @pytest.mark.parametrize("M,K", [(1, 8), (2, 64), (3, 1000), (5, 4096), (2, 8200), (33, 1155)])
@@ -132,7 +137,7 @@ def test_packed_weight_and_its_transpose(N, K, dtype):
 
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------
-SIZES = [(1, 1, 1), (1, 129, 127), (1, 4096, 4096), (3, 64, 128), (8, 96, 640), (16, 200, 1000), (17, 130, 257), (33, 1000, 640), (65, 1, 512),
+SIZES = [(1, 1, 1), (16, 100, 4096), (16, 100, 4100), (9, 260, 8192), (1, 50, 65536), (2, 33, 65537), (1, 129, 127), (1, 4096, 4096), (3, 64, 128), (8, 96, 640), (16, 200, 1000), (17, 130, 257), (33, 1000, 640), (65, 1, 512),
          (64, 300, 640), (77, 768, 768), (129, 257, 385), (300, 65, 1152), (255, 513, 130), (700, 520, 200), (1000, 1030, 129)]
 
 
@@ -157,7 +162,10 @@ def test_product(M, N, K, xt, yt):
     xv, wv = R.quantise(_np(x))[0], R.quantise(_np(w), 128)[0]
     ref = xv @ wv.T
     X = x.cuda()
-    _check(ops.gemm_fp8(X, W, out_f32=yt == F32), ref, xv, wv, yt)
+    y = ops.gemm_fp8(X, W, out_f32=yt == F32)
+    _check(y, ref, xv, wv, yt)
+    if M <= 16:                                                       # quantised inside the product: the same codes
+        assert torch.equal(y, ops.gemm_fp8(ops.quant_fp8(X), W, out_f32=yt == F32))
     _check(ops.gemm_fp8(ops.quant_fp8(X), W, bias=b.cuda(), residual=r.cuda(), out_f32=yt == F32), ref + _np(b) + _np(r), xv, wv, yt,
            add=np.abs(_np(b)) + np.abs(_np(r)))
 
