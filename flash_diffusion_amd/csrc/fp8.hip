@@ -820,7 +820,7 @@ int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st) {
     if (a.x_f32) return a.out_f32 ? launch_stream<1, 1, true, float>(a, st) : launch_stream<1, 1, false, float>(a, st);
     return a.out_f32 ? launch_stream<1, 1, true, bf16_t>(a, st) : launch_stream<1, 1, false, bf16_t>(a, st);
   }
-  if (a.H) return a.M <= 64 ? launch_tile<64, 256, 1, 4, true, false, true>(a, st) : launch_tile<128, 256, 2, 4, true, false, true>(a, st);
+  if (a.H) return ((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 128 ? launch_tile<64, 256, 1, 4, true, false, true>(a, st) : launch_tile<128, 256, 2, 4, true, false, true>(a, st);
   const int es = a.out_f32 ? 4 : 2;
   const bool vec = a.N % 8 == 0 && aligned(a.C, a.ldc * es, 16) && (!a.residual || aligned(a.residual, a.ldr * es, 16)) && ((uintptr_t)a.bias & 15) == 0;
   static const Fp8Cost narrow[] = {{64, 64, .09, .172, 3., .5}, {128, 128, .02, .46, 3., 1.}, {128, 256, 0., .86, 3., 3.}, {256, 256, 0., 1.45, 3., 5.}};

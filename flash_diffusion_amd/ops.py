@@ -465,14 +465,25 @@ def _untile(codes, rows, K):
 
 class Fp8Rows:
     """Rows of activations [M, K] in 8 bits: e4m3 codes in tiles, a power-of-two scale for each row and 128 columns (include/fdmi.h has the
-    layout).  .values() reads them back."""
-    __slots__ = ("M", "K", "codes", "scales")
+    layout; `data` holds the codes and behind them the scales).  .values() reads them back."""
+    __slots__ = ("M", "K", "data", "cut")
 
     def __init__(self, M, K, device):
         self.M, self.K = M, K
-        Mp, Kb = _pad(M, 16), _pad(K, 128) // 128
-        b = torch.empty(Mp * Kb * 129, dtype=torch.uint8, device=device)
-        self.codes, self.scales = b[:Mp * Kb * 128], b[Mp * Kb * 128:]
+        self.cut = _pad(M, 16) * _pad(K, 128)
+        self.data = torch.empty(self.cut // 128 * 129, dtype=torch.uint8, device=device)
+
+    def pointers(self):
+        p = self.data.data_ptr()
+        return p, p + self.cut
+
+    @property
+    def codes(self):
+        return self.data[:self.cut]
+
+    @property
+    def scales(self):
+        return self.data[self.cut:]
 
     def parts(self):
         """(codes [M, K] e4m3, scales [M, ceil(K / 128)] e8m0): a value is its code times its block's scale"""
@@ -530,8 +541,9 @@ def rmsnorm_fp8(x, w, eps):
     if K < 1:
         raise ValueError(f"x has no columns: {tuple(x.shape)}")
     o = Fp8Rows(M, K, x.device)
-    check(lib().fdmi_quant_fp8(x.data_ptr(), x.dtype == F32, ld, None if w is None else _vector(w, K, "w"), eps, o.codes.data_ptr(),
-                               o.scales.data_ptr(), M, K, _stream()))
+    codes, scales = o.pointers()
+    check(lib().fdmi_quant_fp8(x.data_ptr(), x.dtype == F32, ld, None if w is None else _vector(w, K, "w"), eps, codes, scales, M, K,
+                               _stream()))
     return o
 
 
@@ -541,8 +553,9 @@ def _fp8_rows_of(d, A, K, what, gated=False):
     if isinstance(A, Fp8Rows):
         if A.K != K:
             raise ValueError(f"{what} has {A.K} columns, the weight contracts over {K}")
-        d.M, d.X, d.sx = A.M, _here(A.codes, what).data_ptr(), A.scales.data_ptr()
-        return A.codes
+        _here(A.data, what)
+        d.M, (d.X, d.sx) = A.M, A.pointers()
+        return A.data
     d.ldxr = _rows(A, what)
     M, cols = A.shape
     if cols != K:
@@ -608,7 +621,7 @@ def gated_fp8(A, W, W2):
     d.N, d.K = W.N, W.K
     d.W, d.sw = _here(W.codes, "weight").data_ptr(), W.scales.data_ptr()
     d.W2, d.sw2 = _here(W2.codes, "second weight").data_ptr(), W2.scales.data_ptr()
-    d.H, d.sh = o.codes.data_ptr(), o.scales.data_ptr()
+    d.H, d.sh = o.pointers()
     if d.M:
         check(lib().fdmi_gemm_fp8(C.byref(d), _stream()))
     return o
