@@ -20,6 +20,7 @@ import torch.nn as nn
 
 from . import ops
 from .conditioners import BaseConditioner
+from .fp8 import TokenEmbedding
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -68,7 +69,7 @@ class _Layer(nn.Module):
 class _Embeddings(nn.Module):
     def __init__(self, vocab, d, maxpos):
         super().__init__()
-        self.token_embedding = nn.Embedding(vocab, d)
+        self.token_embedding = TokenEmbedding(vocab, d)
         self.position_embedding = nn.Embedding(maxpos, d)
         self.register_buffer("position_ids", torch.arange(maxpos).unsqueeze(0), persistent=False)
 
@@ -118,10 +119,16 @@ class MiCLIPTextModel(nn.Module):
         B, S = input_ids.shape
         D, H = c.hidden_size, c.num_attention_heads
         emb = tm.embeddings
-        h32 = emb.token_embedding.weight[input_ids] + emb.position_embedding.weight[emb.position_ids[0, :S]][None]   # [B, S, D] f32
-        h = self._act(h32.reshape(B * S, D).contiguous())
-        hidden: List[torch.Tensor] = [h32.reshape(B, S, D)] if output_hidden_states else []
-        eps, dt = c.layer_norm_eps, self.dt
+        dt = self.dt
+        pos = emb.position_embedding.weight[:S].float()
+        hidden: List[torch.Tensor] = []
+        if output_hidden_states:               # hidden_states[0] is the embedding in fp32
+            h32 = emb.token_embedding(input_ids, pos=pos, dtype=F32)
+            hidden.append(h32)
+            h = self._act(h32.view(B * S, D))
+        else:
+            h = emb.token_embedding(input_ids, pos=pos, dtype=dt).view(B * S, D)
+        eps = c.layer_norm_eps
         for lyr in tm.encoder.layers:
             a = lyr.self_attn
             n1 = ops.layernorm_fwd(h, lyr.layer_norm1.weight, lyr.layer_norm1.bias, eps)

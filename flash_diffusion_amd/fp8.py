@@ -1,0 +1,130 @@
+"""Layers over the 8-bit products and the embedding lookup (csrc/fp8.hip, csrc/embed.hip): ``Fp8Linear``, a frozen linear map whose input
+gradient flows, ``TokenEmbedding``, ``nn.Embedding``'s lookup and sparse-by-nature gradient on the HIP path, and ``PackedFp8``, the
+cache through which a module keeps the 8-bit form of a parameter (the frozen text encoder of ``t5.py`` with precision="fp8").
+
+What trains in front of a frozen 8-bit encoder layer is a token table (textual inversion): its gradient is the products' input gradient
+summed by token.  The weights themselves are frozen: there is no weight gradient.  GPU only; there is no CPU fallback."""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from . import ops
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+class PackedFp8:
+    """The 8-bit form of ONE parameter, packed on first use and again when the parameter has changed (replaced, moved, or written in place:
+    torch counts those).  The parameter itself is held, so another one at the same address is not taken for it.  Streams other than
+    the one it was packed on wait for the packing; a capture cannot pack (run the layer once before)."""
+
+    def __init__(self, transposed=False):
+        self.transposed = transposed
+        self._of = self._key = self._packed = self._event = self._stream = None
+
+    def __deepcopy__(self, memo):
+        return PackedFp8(self.transposed)          # (the copy's parameter is another one)
+
+    def __reduce__(self):
+        return PackedFp8, (self.transposed,)
+
+    def __call__(self, w):
+        key = (w._version, w.data_ptr(), w.device, w.dtype, tuple(w.shape))
+        capturing = torch.cuda.is_current_stream_capturing()
+        if self._of is not w or self._key != key:
+            if capturing:
+                raise RuntimeError("the weight has to be packed before a graph is captured: run the layer once")
+            if self._packed is not None:
+                torch.cuda.synchronize()           # (a stream may still read the codes that are dropped here)
+            packed, stream, event = ops.pack_weight_fp8(w.detach().contiguous(), self.transposed), torch.cuda.current_stream(), torch.cuda.Event()
+            event.record(stream)
+            self._packed, self._stream, self._event = packed, stream, event
+            self._key, self._of = key, w
+        elif self._event is not None and not capturing:   # (a capture begins with a synchronisation of the device)
+            if self._event.query():
+                self._event = None
+            elif torch.cuda.current_stream() != self._stream:
+                torch.cuda.current_stream().wait_event(self._event)
+        return self._packed
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, packed, bias, out_f32):
+        ctx.packed, ctx.shape, ctx.dtype = packed, x.shape, x.dtype
+        y = ops.gemm_fp8(x.reshape(-1, x.shape[-1]), packed, bias=bias, out_f32=out_f32)
+        return y.view(*x.shape[:-1], packed.N)
+
+    @staticmethod
+    def backward(ctx, dy):
+        dy = dy.reshape(-1, dy.shape[-1])
+        if dy.shape[1] > 1 and dy.stride(1) != 1 or dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]:
+            dy = dy.contiguous()                    # (a broadcast gradient, e.g. that of a sum)
+        dx = ops.gemm_fp8_dgrad(dy, ctx.packed, out_f32=ctx.dtype == F32)
+        return dx.view(ctx.shape), None, None, None
+
+
+class Fp8Linear(nn.Module):
+    """``nn.Linear`` with a frozen weight held in 8 bits (ops.pack_weight_fp8) and a frozen fp32 bias: y = x W^T + b for bf16 / fp32 inputs of
+    any leading shape, in the input's dtype.  The gradient flows to the input; its dY is quantised like an activation."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor = None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        packed = ops.pack_weight_fp8(weight.detach(), transposed=True)
+        for name in self._PARTS:
+            self.register_buffer(name, getattr(packed, name))
+        self.register_buffer("bias", None if bias is None else bias.detach().to(weight.device, F32).contiguous())
+
+    _PARTS = ("codes", "scales", "codes_t", "scales_t")
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear):
+        return cls(linear.weight, linear.bias)
+
+    def packed(self):
+        """the weight as the ops take it (the buffers move and are saved with the module)"""
+        w = ops.Fp8Weight.__new__(ops.Fp8Weight)
+        w.N, w.K = self.out_features, self.in_features
+        for name in self._PARTS:
+            setattr(w, name, getattr(self, name))
+        return w
+
+    def forward(self, x):
+        return _Fp8LinearFn.apply(x, self.packed(), None if self.bias is None else self.bias.float(), x.dtype == F32)
+
+
+class _LookupFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, pos, ids, scale, dtype):
+        ctx.save_for_backward(ids)
+        ctx.V, ctx.scale, ctx.wdtype = weight.shape[0], scale, weight.dtype
+        ctx.pos_rows = None if pos is None else pos.shape[0]
+        return ops.embed_fwd(weight, ids, scale=scale, pos=pos, dtype=dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        dy = dy.contiguous()
+        dw = dp = None
+        if ctx.needs_input_grad[0]:
+            dw = ops.embed_bwd(dy, ids, ctx.V, scale=ctx.scale).to(ctx.wdtype)
+        if ctx.needs_input_grad[1]:                # the position rows are a lookup too, by the last index of ids
+            t = torch.arange(ids.shape[-1] if ids.dim() else 1, dtype=torch.int32, device=ids.device).expand(ids.shape).contiguous()
+            dp = ops.embed_bwd(dy, t, ctx.pos_rows)
+        return dw, dp, None, None, None
+
+
+class TokenEmbedding(nn.Embedding):
+    """``nn.Embedding`` (same parameter, same state_dict) whose lookup is ops.embed_fwd -- scale * weight[ids] + pos[t] in one pass, rounded
+    once to `dtype` -- and whose gradient is ops.embed_bwd's (fixed order of sums).  The options of nn.Embedding that change either
+    (padding_idx, max_norm, scale_grad_by_freq, sparse) are refused.  An id outside the table gives a row of NaN."""
+
+    def __init__(self, num_embeddings, embedding_dim, **kw):
+        super().__init__(num_embeddings, embedding_dim, **kw)
+        if self.padding_idx is not None or self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise NotImplementedError("TokenEmbedding: padding_idx, max_norm, scale_grad_by_freq and sparse are not implemented")
+
+    def forward(self, ids, scale=1.0, pos=None, dtype=BF16):
+        return _LookupFn.apply(self.weight, pos, ids, float(scale), dtype)

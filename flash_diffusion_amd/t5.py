@@ -12,9 +12,13 @@ The arithmetic is upstream T5 (v1.0 ``relu`` and v1.1 / flan ``gated-gelu``): T5
 attention whose scores receive the bucketed relative-position bias of block 0 (shared by all blocks) and the additive key mask,
 ``h += o(attn)``, gated feed-forward ``wo(gelu_new(wi_0 x) * wi_1 x)``, final T5LayerNorm.  Every token-major operation is a launch of
 libfdmi.so's op-level C-ABI: ``fdmi_rmsnorm``, bf16 MFMA GEMMs (tanh-GELU and the residual in the epilogues), ``fdmi_mul``, and the
-biased attention through the exact-f32 materialised-score kernels (``fdmi_attn_bias_fwd_f32``; 120 keys: the cost is nil).  torch does
-the embedding lookup and builds the [H, S, S] bias table from the bucket embedding (integer bucketing of S x S positions, cached per
-S).  GPU only; there is no CPU fallback."""
+biased attention through the exact-f32 materialised-score kernels (``fdmi_attn_bias_fwd_f32``; 120 keys: the cost is nil), the token lookup
+``fdmi_embed_fwd``.  torch builds the [H, S, S] bias table from the bucket embedding (integer bucketing of S x S positions, cached per
+S).  GPU only; there is no CPU fallback.
+
+precision="fp8": the bf16 encoder with every projection as an 8-bit product (csrc/fp8.hip: e4m3 codes, a power-of-two scale for each 128
+columns of a row and each 128 x 128 block of a weight): both norms quantise their result, the gated feed-forward hands its product
+on as codes, residual stream and attention as in bf16.  Half the weight bytes of bf16 once packed."""
 from __future__ import annotations
 
 import math
@@ -26,6 +30,7 @@ import torch.nn as nn
 
 from . import ops
 from .conditioners import BaseConditioner
+from .fp8 import PackedFp8, TokenEmbedding
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -37,6 +42,7 @@ class _W(nn.Module):
         super().__init__()
         self.weight = nn.Parameter(torch.randn(out_f, in_f) * in_f ** -0.5)
         self._cache = None
+        self.operand8 = PackedFp8()
 
     def operand(self, dt):
         w = self.weight
@@ -91,7 +97,7 @@ class _Block(nn.Module):
 class _Stack(nn.Module):
     def __init__(self, vocab, d, inner, heads, ff, gated, n, buckets):
         super().__init__()
-        self.embed_tokens = nn.Embedding(vocab, d)
+        self.embed_tokens = TokenEmbedding(vocab, d)
         self.block = nn.ModuleList([_Block(d, inner, heads, ff, gated, buckets if i == 0 else 0) for i in range(n)])
         self.final_layer_norm = _Norm(d)
 
@@ -112,15 +118,16 @@ class MiT5EncoderModel(nn.Module):
                  relative_attention_num_buckets=32, relative_attention_max_distance=128, layer_norm_epsilon=1e-6,
                  feed_forward_proj="gated-gelu", precision="bf16", **unused):
         super().__init__()
-        assert precision in ("bf16", "fp32") and feed_forward_proj in ("gated-gelu", "relu"), (precision, feed_forward_proj)
+        assert precision in ("bf16", "fp32", "fp8") and feed_forward_proj in ("gated-gelu", "relu"), (precision, feed_forward_proj)
         inner = d_kv * num_heads
         assert d_model % 8 == 0 and inner % 8 == 0 and d_ff % 8 == 0
         self.dt = F32 if precision == "fp32" else BF16
+        self.fp8 = precision == "fp8"
         self.config = SimpleNamespace(vocab_size=vocab_size, d_model=d_model, d_kv=d_kv, d_ff=d_ff, num_layers=num_layers,
                                       num_heads=num_heads, relative_attention_num_buckets=relative_attention_num_buckets,
                                       relative_attention_max_distance=relative_attention_max_distance,
                                       layer_norm_epsilon=layer_norm_epsilon, feed_forward_proj=feed_forward_proj)
-        self.shared = nn.Embedding(vocab_size, d_model)
+        self.shared = TokenEmbedding(vocab_size, d_model)
         self.encoder = _Stack(vocab_size, d_model, inner, num_heads, d_ff, feed_forward_proj == "gated-gelu", num_layers,
                               relative_attention_num_buckets)
         self.encoder.embed_tokens.weight = self.shared.weight          # tied, as in transformers
@@ -145,15 +152,50 @@ class MiT5EncoderModel(nn.Module):
             self._bias_cache = (key, w.detach().float()[bucket].permute(2, 0, 1).contiguous())                 # [H, S, S]
         return self._bias_cache[1]
 
+    def _block(self, blk, h, B, S, bias, kbias):
+        c, dt, eps = self.config, self.dt, self.config.layer_norm_epsilon
+        H, inner = c.num_heads, c.d_kv * c.num_heads
+        sa, ff = blk.layer[0], blk.layer[1]
+        a = sa.SelfAttention
+        n1 = ops.rmsnorm(h, sa.layer_norm.weight, eps)
+        q = ops.gemm(n1, a.q.operand(dt), out_f32=True).view(B, S, inner)
+        k = ops.gemm(n1, a.k.operand(dt), out_f32=True).view(B, S, inner)
+        v = ops.gemm(n1, a.v.operand(dt), out_f32=True).view(B, S, inner)
+        o = ops.attn_bias_fwd(q, k, v, H, 1.0, bias, kbias).view(B * S, inner)     # T5 does not scale the scores
+        h = ops.gemm(self._act(o), a.o.operand(dt), residual=h)
+        n2 = ops.rmsnorm(h, ff.layer_norm.weight, eps)
+        dn = ff.DenseReluDense
+        if c.feed_forward_proj == "gated-gelu":
+            f = ops.mul(ops.gemm(n2, dn.wi_0.operand(dt), act=ops.ACT_GELU_TANH), ops.gemm(n2, dn.wi_1.operand(dt)))
+        else:
+            f = ops.gemm(n2, dn.wi.operand(dt), act=ops.ACT_RELU)
+        return ops.gemm(f, dn.wo.operand(dt), residual=h)
+
+    def _block8(self, blk, h, B, S, bias, kbias):
+        """the same block with 8-bit products; its norms and the gated product leave as codes"""
+        c, eps = self.config, self.config.layer_norm_epsilon
+        H, inner = c.num_heads, c.d_kv * c.num_heads
+        sa, ff = blk.layer[0], blk.layer[1]
+        a, dn = sa.SelfAttention, ff.DenseReluDense
+        w8 = lambda m: m.operand8(m.weight)
+        n1 = ops.rmsnorm_fp8(h, sa.layer_norm.weight, eps)
+        q, k, v = (ops.gemm_fp8(n1, w8(m)).view(B, S, inner) for m in (a.q, a.k, a.v))
+        o = ops.attn_bias_fwd(q, k, v, H, 1.0, bias, kbias).view(B * S, inner)
+        h = ops.gemm_fp8(o, w8(a.o), residual=h)
+        n2 = ops.rmsnorm_fp8(h, ff.layer_norm.weight, eps)
+        if c.feed_forward_proj == "gated-gelu":
+            f = ops.gated_fp8(n2, w8(dn.wi_0), w8(dn.wi_1))
+        else:
+            f = ops.gemm_fp8(n2, w8(dn.wi), act=ops.ACT_RELU)
+        return ops.gemm_fp8(f, w8(dn.wo), residual=h)
+
     @torch.no_grad()
     def forward(self, input_ids, attention_mask=None, output_hidden_states=False, **kw):
         c = self.config
         assert input_ids.is_cuda, "MiT5EncoderModel runs on the GPU only (no CPU fallback)"
         B, S = input_ids.shape
-        D, H, dt, eps = c.d_model, c.num_heads, self.dt, c.layer_norm_epsilon
-        inner = c.d_kv * H
-        h32 = self.shared.weight[input_ids]                                                                   # [B, S, D] f32
-        h = self._act(h32.reshape(B * S, D).contiguous())
+        D, dt, eps = c.d_model, self.dt, c.layer_norm_epsilon
+        h = self.shared(input_ids, dtype=dt).view(B * S, D)
         hidden: List[torch.Tensor] = []
         bias = self._position_bias(S, input_ids.device)
         kbias = None
@@ -162,21 +204,7 @@ class MiT5EncoderModel(nn.Module):
         for blk in self.encoder.block:
             if output_hidden_states:
                 hidden.append(h.float().view(B, S, D))
-            sa, ff = blk.layer[0], blk.layer[1]
-            a = sa.SelfAttention
-            n1 = ops.rmsnorm(h, sa.layer_norm.weight, eps)
-            q = ops.gemm(n1, a.q.operand(dt), out_f32=True).view(B, S, inner)
-            k = ops.gemm(n1, a.k.operand(dt), out_f32=True).view(B, S, inner)
-            v = ops.gemm(n1, a.v.operand(dt), out_f32=True).view(B, S, inner)
-            o = ops.attn_bias_fwd(q, k, v, H, 1.0, bias, kbias).view(B * S, inner)     # T5 does not scale the scores
-            h = ops.gemm(self._act(o), a.o.operand(dt), residual=h)
-            n2 = ops.rmsnorm(h, ff.layer_norm.weight, eps)
-            dn = ff.DenseReluDense
-            if c.feed_forward_proj == "gated-gelu":
-                f = ops.mul(ops.gemm(n2, dn.wi_0.operand(dt), act=ops.ACT_GELU_TANH), ops.gemm(n2, dn.wi_1.operand(dt)))
-            else:
-                f = ops.gemm(n2, dn.wi.operand(dt), act=ops.ACT_RELU)
-            h = ops.gemm(f, dn.wo.operand(dt), residual=h)
+            h = (self._block8 if self.fp8 else self._block)(blk, h, B, S, bias, kbias)
         last = ops.rmsnorm(h, self.encoder.final_layer_norm.weight, eps).float().view(B, S, D)
         if output_hidden_states:
             hidden.append(last)

@@ -95,3 +95,30 @@ def test_the_reference_quantiser_agrees_with_torchs_cast():
     m = np.abs(np.pad(x.numpy(), ((0, 0), (0, 68))).reshape(9, 6, 128)).max(2)
     sc = 2.0 ** exps.astype(np.float64)
     assert (m <= 448 * sc).all() and (m > 224 * sc).all()
+
+
+def test_layers_refuse_what_they_do_not_implement_and_caches_copy_empty():
+    import copy
+    import pickle
+    from flash_diffusion_amd.fp8 import PackedFp8, TokenEmbedding
+    for kw in (dict(padding_idx=0), dict(max_norm=1.0), dict(scale_grad_by_freq=True), dict(sparse=True)):
+        with pytest.raises(NotImplementedError):
+            TokenEmbedding(10, 4, **kw)
+    assert set(TokenEmbedding(10, 4).state_dict()) == {"weight"}
+    p = PackedFp8(transposed=True)
+    p._of = object()
+    for c in (copy.deepcopy(p), pickle.loads(pickle.dumps(p))):
+        assert c.transposed and c._of is None
+
+
+def test_t5_and_clip_keep_their_state_dict_names_and_modes():
+    from flash_diffusion_amd.clip import MiCLIPTextModel
+    from flash_diffusion_amd.t5 import MiT5EncoderModel
+    kw = dict(vocab_size=20, d_model=16, d_kv=8, d_ff=24, num_layers=1, num_heads=2)
+    for precision in ("bf16", "fp32", "fp8"):
+        sd = MiT5EncoderModel(**kw, precision=precision).state_dict()
+        assert {"shared.weight", "encoder.embed_tokens.weight", "encoder.block.0.layer.1.DenseReluDense.wi_1.weight"} <= set(sd)
+        assert not any("operand8" in k for k in sd)
+    with pytest.raises(AssertionError):
+        MiT5EncoderModel(**kw, precision="int8")
+    assert "text_model.embeddings.token_embedding.weight" in MiCLIPTextModel(vocab_size=20, hidden_size=16, intermediate_size=24, num_hidden_layers=1, num_attention_heads=2).state_dict()
