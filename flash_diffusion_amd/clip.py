@@ -8,8 +8,8 @@ transformers' state_dict names (``text_model.embeddings.token_embedding.weight``
 
 Every token-major operation is a launch of libfdmi.so's op-level C-ABI: LayerNorm (affine), bf16 MFMA GEMMs with fused bias /
 residual / activation epilogues (quick-GELU as SiLU(1.702 x) / 1.702 folded into the two MLP GEMMs' alpha, exact GELU as its own
-epilogue), causal self-attention through the exact-f32 materialised-score kernels (77 tokens: the cost is nil).  torch does the
-embedding lookup (a gather on parameters) and the pooled-row selection.  GPU only."""
+epilogue), causal self-attention through the exact-f32 materialised-score kernels (77 tokens: the cost is nil), the token and position
+embeddings by the lookup kernel.  torch does the pooled-row selection.  GPU only."""
 from __future__ import annotations
 
 from types import SimpleNamespace

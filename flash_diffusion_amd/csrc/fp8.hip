@@ -9,8 +9,8 @@
 // infinity, and a saturated code would hide the overflow) and the block's scale comes from its finite values.
 //
 // Codes lie in tiles of 16 rows x 64 columns, 1 KiB each: [row tile][column tile][chunk of 16 columns][row][16 bytes].  One wave's load, store or
-// LDS transfer moves whole tiles (row-major codes fill LDS at two thirds of that rate: 128 x 128 tiles of an 8192^3 product in 627 against
-// 499 us), a matrix fragment is one 16-byte read per lane and tile, and the 16 lanes that LDS serves at once read 256 consecutive bytes.
+// LDS transfer moves whole tiles (row-major codes fill LDS at two thirds of that rate: the first 128 x 128 kernel took 627 us over them for 8192^3
+// against 499), a matrix fragment is one 16-byte read per lane and tile, and the 16 lanes that LDS serves at once read 256 consecutive bytes.
 // Scale bytes of activations: [block of 128 columns][rows padded to 16]; of weights: [block][groups of 32 rows].  Weights are padded with
 // zeros to 256 rows, so a tile's loads need no bounds there.
 #include "fp8.h"
@@ -254,8 +254,20 @@ __device__ __forceinline__ float act_of(int act, float v) {
   }
 }
 
-// eight consecutive columns of one row: + bias + residual, activation, 16-byte stores.  Rows of C, the residual and the bias are aligned
-__device__ __forceinline__ void store8(const Fp8GemmArgs& a, int m, int n, float v[8]) {
+// eight consecutive columns of one row, with 16-byte accesses: the residual (16 bytes of bf16, 32 of fp32) ...
+template <bool F32>
+__device__ __forceinline__ void load_res8(const Fp8GemmArgs& a, int m, int n, uint4 r[F32 ? 2 : 1]) {
+  if constexpr (F32) {
+    const uint4* p = (const uint4*)((const float*)a.residual + (int64_t)m * a.ldr + n);
+    r[0] = p[0];
+    r[1] = p[1];
+  } else {
+    r[0] = *(const uint4*)((const bf16_t*)a.residual + (int64_t)m * a.ldr + n);
+  }
+}
+// ... and sums + bias, activation, + residual, stored.  Rows of C, the residual and the bias are aligned
+template <bool F32>
+__device__ __forceinline__ void store8(const Fp8GemmArgs& a, int m, int n, float v[8], const uint4 r[F32 ? 2 : 1]) {
   if (a.bias) {
     const float4 p = *(const float4*)(a.bias + n), q = *(const float4*)(a.bias + n + 4);
     v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w; v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
@@ -264,23 +276,24 @@ __device__ __forceinline__ void store8(const Fp8GemmArgs& a, int m, int n, float
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = act_of(a.act, v[i]);
   }
-  if (a.out_f32) {
+  if constexpr (F32) {
     float* c = (float*)a.C + (int64_t)m * a.ldc + n;
     if (a.residual) {
-      const float* r = (const float*)a.residual + (int64_t)m * a.ldr + n;
-      const float4 p = *(const float4*)r, q = *(const float4*)(r + 4);
-      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w; v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
+      v[0] += __uint_as_float(r[0].x); v[1] += __uint_as_float(r[0].y); v[2] += __uint_as_float(r[0].z); v[3] += __uint_as_float(r[0].w);
+      v[4] += __uint_as_float(r[1].x); v[5] += __uint_as_float(r[1].y); v[6] += __uint_as_float(r[1].z); v[7] += __uint_as_float(r[1].w);
     }
     *(float4*)c = make_float4(v[0], v[1], v[2], v[3]);
     *(float4*)(c + 4) = make_float4(v[4], v[5], v[6], v[7]);
   } else {
-    bf16_t* c = (bf16_t*)a.C + (int64_t)m * a.ldc + n;
     if (a.residual) {
-      const u16x8 t = *(const u16x8*)((const bf16_t*)a.residual + (int64_t)m * a.ldr + n);
+      const uint32_t t[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += bf2f(t[i]);
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] += __uint_as_float(t[i] << 16);
+        v[2 * i + 1] += __uint_as_float(t[i] & 0xffff0000u);
+      }
     }
-    *(uint4*)c = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+    *(uint4*)((bf16_t*)a.C + (int64_t)m * a.ldc + n) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
   }
 }
 __device__ __forceinline__ void store1(const Fp8GemmArgs& a, int m, int n, float v) {
@@ -308,6 +321,7 @@ __device__ __forceinline__ void store1(const Fp8GemmArgs& a, int m, int n, float
 // ring runs on into the next item, so a tile's epilogue is spent with the next tile's first stages on their way (a launch of one
 // workgroup per tile lost 11 us a tile at 256 x 256 x 4096).  An item's scale bytes are fetched during the item before, into the other of
 // two panels.  The last tile row is moved up to end at the last row of X; the rows it shares with its neighbour are not stored twice.
+constexpr int BAND = 4;                                               // tile rows walked together (4 and 8 measure alike)
 constexpr int SEG = 48;                                              // blocks of 128 per item
 constexpr int fp8_segments(int kb) { return (kb + SEG - 1) / SEG; }
 constexpr int fp8_segment(int kb) { return (kb + fp8_segments(kb) - 1) / fp8_segments(kb); }
@@ -332,14 +346,14 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
   const int Mt = (a.M + 15) >> 4, len = fp8_segment(a.Kb);
   const int64_t Mp = (int64_t)Mt * 16, Ng = (int64_t)((a.N + 255) >> 8) * 8;
 
-  // block b runs on XCD b % 8: give each XCD a contiguous range of tiles of a column-first walk through bands of eight tile rows (the
-  // tiles in flight on an XCD share eight panels of X and a few of W)
+  // block b runs on XCD b % 8: give each XCD a contiguous range of tiles of a column-first walk through bands of BAND tile rows (the
+  // tiles in flight on an XCD share a few panels of X and of W)
   struct Item { int v, m0, mt, n0, kb0, stages; };                    // mt: first row tile of X that is loaded
   auto place = [&](Item& it) {
     const int xcd = it.v & 7, qd = total >> 3, rem = total & 7;
     const int t = (xcd < rem ? xcd * (qd + 1) : rem * (qd + 1) + (xcd - rem) * qd) + (it.v >> 3);
-    const int band = t / (8 * tilesN), in = t - band * 8 * tilesN, rows = tilesM - band * 8 < 8 ? tilesM - band * 8 : 8;
-    it.m0 = (band * 8 + in % rows) * BM;
+    const int band = t / (BAND * tilesN), in = t - band * BAND * tilesN, rows = tilesM - band * BAND < BAND ? tilesM - band * BAND : BAND;
+    it.m0 = (band * BAND + in % rows) * BM;
     it.n0 = (in / rows) * BN;
     it.mt = it.m0 >> 4;
     if (it.mt > Mt - BM / 16) it.mt = Mt > BM / 16 ? Mt - BM / 16 : 0;
@@ -473,9 +487,24 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
       }
       __syncthreads();                                                // (red is written again by the next tile)
     } else if constexpr (VEC) {
-      // lanes l and l + 32 hold alternating runs of four columns: exchange so that each has eight consecutive ones
+      // lanes l and l + 32 hold alternating runs of four columns: exchange so that each has eight consecutive ones.  The residual of the next
+      // 32 rows is asked for before these are stored (C may be the residual, so the compiler keeps loads behind the stores before them;
+      // 8192^3 with a residual: 457 us without, 441 with the loads ahead)
+      uint4 res[2][NF][2][WIDE ? 2 : 1];
+      auto fetch = [&](int k) {
+        const int m = mw + k * 32 + j;
+#pragma unroll
+        for (int i = 0; i < NF; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int n = nw + i * 32 + r * 16 + half * 8;
+            if (m >= it.m0 && m < a.M && n < a.N) load_res8<WIDE>(a, m, n, res[k & 1][i][r]);
+          }
+      };
+      if (a.residual) fetch(0);
 #pragma unroll
       for (int k = 0; k < MF; ++k) {
+        if (a.residual && k + 1 < MF) fetch(k + 1);
         const int m = mw + k * 32 + j;
 #pragma unroll
         for (int i = 0; i < NF; ++i)
@@ -490,7 +519,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
               v[4 + t] = __uint_as_float(e[1]);
             }
             const int n = nw + i * 32 + r * 16 + half * 8;
-            if (m >= it.m0 && m < a.M && n < a.N) store8(a, m, n, v);
+            if (m >= it.m0 && m < a.M && n < a.N) store8<WIDE>(a, m, n, v, res[k & 1][i][r]);
           }
       }
     } else {
@@ -578,9 +607,8 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
         }
         read_step(slot + 2 * kb, s + AHEAD);
         if (s == 0) read_scales(cur, which, kb + 1 < blocks ? kb + 1 : kb);
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MF < 4) __builtin_amdgcn_sched_barrier(0);   // (8192^3: 464 us with it at 128 x 128, 482 without; 256 x 256: 395, 390)
         multiply(s);
-        __builtin_amdgcn_sched_barrier(0);
         const int u = (s + AHEAD) % MF, h = 2 * kb + (s + AHEAD) / MF + 3;   // burst u since the hand-over to stage h - 3
         const int over = h - cur.stages;
         const int64_t in = over >> 31, own = (int64_t)h * 1024, far = (int64_t)over * step;
@@ -797,8 +825,8 @@ int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t
 // on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU rounded up; the streaming kernel is bound by what its workgroups
 // read from L2 (25 TB/s over all CUs; a short grid leaves some idle) or by the weight from memory.  Measured against each other at
 // 8192^3, 1920 x 4096 x {4096, 10240}, {1, 16, 64} x 4096 x 4096, 512 x 1024 x 4096, 120 x 1024 x 2560, 2048 x 2048 x 4096, for example
-// (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 18.4 / 22.9 / -, 4.3;  1920 x 4096 x 4096: 51 / 34.4 / 33.8 / 50, 91;
-// 16384 x 10240 x 4096: 1020 / 626 / 588 / 534, -.
+// (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 15.7 / 22.8 / 36, 4.3;  1920 x 4096 x 4096: 58 / 32.6 / 32.2 / 46, 72;
+// 1920 x 10240 x 4096: 122 / 73.2 / 80.0 / 89, 246;  8192^3: 1002 / 445 / 437 / 381, 2266;  16384 x 10240 x 4096: 1382 / 603 / 582 / 503, 2018.
 struct Fp8Cost { int BM, BN; double block, share, fixed, tile; };
 double fp8_cost(const Fp8GemmArgs& a, const Fp8Cost& c) {
   const double tiles = double((a.M + c.BM - 1) / c.BM) * ((a.N + c.BN - 1) / c.BN), w = (double)(int64_t)((tiles + 255) / 256);
