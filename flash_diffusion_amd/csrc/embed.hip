@@ -3,15 +3,17 @@
 //   forward    out[i][:] = scale * table[ids[i]][:] + pos[i mod pos_rows][:]
 //   gradient   grad[v][:] = scale * sum over { i : ids[i] = v } of dy[i][:]
 //
-// Both are bound by HBM.  The gradient adds in a fixed order (no atomics): positions are ranked by (id, position), one wave sums a chunk of
-// the sorted list, and runs of one token that cross a chunk's edge leave partial rows that a last launch adds in order.  Three
-// launches: zeros together with the ranking, chunk sums, joins (and one before them where the list is long).
+// Both are bound by HBM.  The gradient adds in a fixed order (no atomics): positions are ranked by (id, position), a workgroup sums a chunk
+// of the sorted list, and runs of one token that cross a chunk's edge leave partial rows that a last launch adds in order.  Three
+// launches: the ranking, chunk sums together with the zeros, joins (and one before them where the list is long).  16384 bf16 rows of 4096
+// columns into 32128 fp32 rows, half of them padding: 156 us, 128 of them in the second launch for 725 MB (5.7 TB/s; a copy reaches
+// 4.9, a fill 6.8); 1232 fp32 rows of 768 into 49408: 35 us, 22.5 of them (6.8 TB/s).
 // An id outside the table reads as a row of NaN (a gather cannot raise on the device) and its gradient is dropped.
 #include "fp8.h"
 
 namespace {
 
-constexpr int CHUNK = 16;              // sorted positions summed by one wave: its 16 rows are in flight together
+constexpr int ROWS = 16, CHUNK = 64;   // sorted positions summed by one wave (its rows are in flight together) and by a workgroup
 constexpr int32_t NONE = 0x7fffffff;   // key of an id outside the table: behind all others
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int ids64, int64_t i) {
@@ -72,9 +74,10 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t 
 
 // ---- gradient: the order ---------------------------------------------------------------------------------------------------------------
 // A position's place in the list sorted by (id, position) is the number of keys below its own.  Up to DIRECT positions they are counted
-// one by one (quadratic, but without a launch of its own: 3 us alone at 1 token, 6 at 1232, 17 at 4928).  Longer lists are first sorted
-// in parts of 256; the other parts' counts are then binary searches (16384 positions: 58 us counted directly, 131072: 1180 us).
-constexpr int DIRECT = 4096, PART = 256;
+// one by one (quadratic, but one launch: 4.6 us at 256 positions, 7.4 at 1232, 10.1 at 2048, 18 at 4096, 58 at 16384).  Longer lists are
+// first sorted in parts of 256; the other parts' counts are then binary searches (two launches: 9.1 us at 1232, 9.2 at 2048, 9.7 at 4096,
+// 17.5 at 16384, 98 at 131072; between two launches lies a microsecond).
+constexpr int DIRECT = 2048, PART = 256;
 constexpr int TILE = 4096;             // keys in LDS at a time
 
 __device__ __forceinline__ uint32_t key_of(const void* ids, int ids64, int64_t V, int64_t p) {
@@ -114,27 +117,16 @@ __global__ __launch_bounds__(PART) void part_sort_kernel(const void* ids, int id
   ppos[p0 + r] = (int32_t)p;
 }
 
-// blocks below `rankers` place positions, the others write zeros (the bulk of the bytes, which hides the order)
 template <bool PARTS>
-__global__ __launch_bounds__(256) void order_kernel(const void* ids, int ids64, int64_t n, int64_t V, const uint32_t* pkey, const int32_t* ppos,
-                                                    int rankers, int32_t* sid, int32_t* spos, float* g, int64_t rows, int D, int64_t ldg) {
-  if ((int)blockIdx.x >= rankers) {
-    const int64_t first = ((int64_t)blockIdx.x - rankers) * 256 + threadIdx.x, step = ((int64_t)gridDim.x - rankers) * 256, total = rows * D;
-    if (ldg == D && ((uintptr_t)g & 15) == 0) {
-      for (int64_t u = first; u < total / 4; u += step) ((float4*)g)[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (first < total % 4) g[total / 4 * 4 + first] = 0.f;
-    } else {
-      for (int64_t u = first; u < total; u += step) g[u / D * ldg + u % D] = 0.f;
-    }
-    return;
-  }
+__global__ __launch_bounds__(PARTS ? 1024 : 256) void order_kernel(const void* ids, int ids64, int64_t n, int64_t V, const uint32_t* pkey, const int32_t* ppos,
+                                                    int32_t* sid, int32_t* spos) {
   __shared__ __attribute__((aligned(16))) uint32_t key[TILE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if constexpr (!PARTS) {                        // 64 positions per block, the list shared out over its waves
     __shared__ int32_t part[4][64];
     const int64_t i0 = (int64_t)blockIdx.x * 64, i = i0 + lane;
     const uint32_t mine = i < n ? key_of(ids, ids64, V, i) : 0;
-    const int groups = (int)((n + 63) >> 6);     // (n <= DIRECT = TILE: one tile)
+    const int groups = (int)((n + 63) >> 6);     // (n <= DIRECT <= TILE: one tile)
     for (int p = threadIdx.x; p < groups * 64; p += 256) key[p] = p < n ? key_of(ids, ids64, V, p) : 0xffffffffu;
     __syncthreads();
     int r = 0;
@@ -147,29 +139,34 @@ __global__ __launch_bounds__(256) void order_kernel(const void* ids, int ids64, 
       sid[at] = (int32_t)mine;
       spos[at] = (int32_t)i;
     }
-  } else {                                       // one sorted part per block
-    const int64_t p = (int64_t)blockIdx.x * PART + threadIdx.x;
+  } else {                                       // one sorted part per block; each quarter of it searches every fourth part
+    __shared__ int32_t found[3][PART];
+    const int quarter = threadIdx.x / PART, t = threadIdx.x % PART;
+    const int64_t p = (int64_t)blockIdx.x * PART + t;
     const uint32_t mine = pkey[p];
     const int32_t pos = ppos[p];
     const int parts = (int)((n + PART - 1) / PART);
-    int64_t at = threadIdx.x;
+    int32_t below = 0;
     for (int c0 = 0; c0 < parts; c0 += TILE / PART) {
       const int here = parts - c0 < TILE / PART ? parts - c0 : TILE / PART;
       __syncthreads();
-      for (int q = threadIdx.x; q < here * PART; q += 256) key[q] = pkey[(int64_t)c0 * PART + q];
+      for (int q = threadIdx.x; q < here * PART; q += 1024) key[q] = pkey[(int64_t)c0 * PART + q];
       __syncthreads();
 #pragma unroll 4
-      for (int c = 0; c < here; ++c) {
+      for (int c = quarter; c < here; c += 4) {
         const uint32_t lim = mine + (c0 + c < (int)blockIdx.x ? 1u : 0u);   // equal keys of earlier parts come first
         const uint32_t* k = key + c * PART;
         int lo = 0;
 #pragma unroll
         for (int step = PART / 2; step > 0; step >>= 1) lo += k[lo + step - 1] < lim ? step : 0;
         lo += k[lo] < lim;
-        at += c0 + c == (int)blockIdx.x ? 0 : lo;
+        below += c0 + c == (int)blockIdx.x ? 0 : lo;
       }
     }
-    if (pos < n) {
+    if (quarter) found[quarter - 1][t] = below;
+    __syncthreads();
+    if (quarter == 0 && pos < n) {
+      const int64_t at = (int64_t)t + below + found[0][t] + found[1][t] + found[2][t];
       sid[at] = (int32_t)mine;
       spos[at] = pos;
     }
@@ -193,43 +190,103 @@ __device__ __forceinline__ void put_row(float* o, const float v[VEC], float scal
   }
 }
 
-// ---- second launch: one wave per chunk of the sorted list and 64 VEC columns -------------------------------------------------------------
-// part[c][0]: the run that came in over the chunk's left edge (the whole chunk, if it also leaves over the right one); part[c][1]: the run
-// that begins here and leaves over the right edge
+// ---- second launch: one workgroup per chunk of the sorted list and 64 VEC columns ---------------------------------------------------------
+// Each wave sums the runs among its 16 positions.  Those that cross from wave to wave are joined through LDS, those that cross a chunk's
+// edge leave part[c][0]: the run that came in over the chunk's left edge (the whole chunk, if it also leaves over the right one), and
+// part[c][1]: the run that begins here and leaves over the right edge.
+//
+// The workgroups behind those of the sums write the zeros, the bulk of the bytes: ZROWS rows of the table each, but for the rows of tokens
+// that occur (looked up in the sorted list; each is written once, by its run).
+constexpr int ZROWS = 16;
+template <int VEC>
+__device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const int32_t* sid, int64_t n, int D, float* g, int64_t ldg) {
+  const int lane = threadIdx.x & 63;
+  const int64_t v = v0 + (lane & (ZROWS - 1));
+  int64_t lo = 0, hi = n;                                     // the first position whose key is not below v
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (sid[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  const bool empty = v < V && !(lo < n && sid[lo] == v);
+  uint32_t todo = (uint32_t)__ballot(empty) & ((1u << ZROWS) - 1);
+  for (; todo; todo &= todo - 1) {
+    float* row = g + (v0 + __ffs(todo) - 1) * ldg;
+    for (int c = threadIdx.x * VEC; c < D; c += 256 * VEC) {
+      if constexpr (VEC == 1) row[c] = 0.f;
+      else *(float4*)(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+}
+
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy, const int32_t* sid, const int32_t* spos, int64_t n, int D,
-                                                      int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part) {
-  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t c = unit / col_groups, p0 = c * CHUNK;
-  const int col = ((int)(unit - c * col_groups) * 64 + (threadIdx.x & 63)) * VEC;
-  if (p0 >= n || col >= D) return;
-  const int count = (int)(p0 + CHUNK < n ? CHUNK : n - p0);
-  const int32_t before = p0 > 0 ? sid[p0 - 1] : -1, after = p0 + CHUNK < n ? sid[p0 + CHUNK] : -1;
-  float v[CHUNK][VEC];
-  int32_t id[CHUNK];
+                                                      int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part, int summers,
+                                                      int64_t V) {
+  if ((int)blockIdx.x >= summers) return zero_rows<(VEC > 1 ? 4 : 1)>(((int64_t)blockIdx.x - summers) * ZROWS, V, sid, n, D, g, ldg);
+  __shared__ float head[4][64 * VEC];            // per wave: its share of the run that came in over its left edge
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t c = blockIdx.x / col_groups, p0 = c * CHUNK + wave * ROWS;
+  const int col = ((int)(blockIdx.x - c * col_groups) * 64 + lane) * VEC, mine = col < D ? col : 0;
+  const int count = (int)(p0 + ROWS < n ? ROWS : p0 < n ? n - p0 : 0);
+  int32_t edge[5];                               // the key at each wave's left edge, and behind the chunk
 #pragma unroll
-  for (int q = 0; q < CHUNK; ++q) {
-    const int64_t p = p0 + (q < count ? q : count - 1);
+  for (int q = 0; q < 5; ++q) edge[q] = c * CHUNK + q * ROWS < n ? sid[c * CHUNK + q * ROWS] : -1;
+  const int32_t before = p0 > 0 && count ? sid[p0 - 1] : -1, after = p0 + ROWS < n ? sid[p0 + ROWS] : -1;
+  float v[ROWS][VEC];
+  int32_t id[ROWS];
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q) {
+    const int64_t p = q < count ? p0 + q : n - 1;
     id[q] = sid[p];
-    load_cols<T, VEC>(dy + (int64_t)spos[p] * lddy + col, v[q]);
+    load_cols<T, VEC>(dy + (int64_t)spos[p] * lddy + mine, v[q]);
   }
-  float sum[VEC];
+  float sum[VEC], out[VEC];
+  int32_t leaves = NONE;                         // the run that begins in this wave and leaves it
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
+  for (int k = 0; k < VEC; ++k) sum[k] = out[k] = 0.f;
 #pragma unroll
-  for (int q = 0; q < CHUNK; ++q) {
-    const bool here = q < count, last = q + 1 == count, ends = here && (last || id[q + 1 < CHUNK ? q + 1 : q] != id[q]);
+  for (int q = 0; q < ROWS; ++q) {
+    const bool here = q < count, last = q + 1 == count, ends = here && (last || id[q + 1 < ROWS ? q + 1 : q] != id[q]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sum[k] = here ? sum[k] + v[q][k] : sum[k];
     if (ends) {
       if (id[q] != NONE) {
-        if (id[q] == before) put_row<VEC>(part + (c * 2) * D + col, sum, 1.f, 0);
-        else if (last && id[q] == after) put_row<VEC>(part + (c * 2 + 1) * D + col, sum, 1.f, 0);
-        else put_row<VEC>(g + (int64_t)id[q] * ldg + col, sum, scale, accumulate);
+        if (id[q] == before) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) head[wave][k * 64 + lane] = sum[k];
+        } else if (last && id[q] == after) {
+          leaves = id[q];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) out[k] = sum[k];
+        } else if (col < D) {
+          put_row<VEC>(g + (int64_t)id[q] * ldg + col, sum, scale, accumulate);
+        }
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
     }
+  }
+  __syncthreads();
+  auto add_heads = [&](int from, int32_t run, float s[VEC]) {          // of the waves from `from` on that begin with the run
+#pragma unroll
+    for (int u = 1; u < 4; ++u)
+      if (u >= from && edge[u] == run)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s[k] += head[u][k * 64 + lane];
+  };
+  if (leaves != NONE) {
+    add_heads(wave + 1, leaves, out);
+    if (col < D) {
+      if (edge[4] == leaves) put_row<VEC>(part + (c * 2 + 1) * D + col, out, 1.f, 0);
+      else put_row<VEC>(g + (int64_t)leaves * ldg + col, out, scale, accumulate);
+    }
+  }
+  if (wave == 0 && before == edge[0] && before != NONE) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) out[k] = head[0][k * 64 + lane];
+    add_heads(1, before, out);
+    if (col < D) put_row<VEC>(part + (c * 2) * D + col, out, 1.f, 0);
   }
 }
 
@@ -239,31 +296,32 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy,
 constexpr int SHORT = 16, JOINERS = 16;
 template <int VEC>
 __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* sid, int64_t n, int D, float scale, int accumulate, float* g,
-                                                                int64_t ldg, const float* part) {
+                                                                   int64_t ldg, const float* part) {
   __shared__ float share[JOINERS][64 * VEC];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = (blockIdx.y * 64 + lane) * VEC;
-  const int64_t chunks = (n + CHUNK - 1) / CHUNK, c = (int64_t)blockIdx.x * JOINERS + lane, p1 = (c + 1) * CHUNK;
-  bool mine = false, far = false;
-  if (lane < JOINERS && p1 < n) {
-    const int32_t id = sid[p1 - 1];
-    mine = id != NONE && sid[p1] == id && (c == 0 || sid[c * CHUNK - 1] != id);
-    far = mine && (c + 1 + SHORT) < chunks && sid[(c + 1 + SHORT) * CHUNK] == id;
-  }
-  uint64_t todo = __ballot(mine), longs = __ballot(far);
+  const int64_t chunks = (n + CHUNK - 1) / CHUNK, k0 = (int64_t)blockIdx.x * JOINERS, c = k0 + (lane & (JOINERS - 1));
+  auto key = [&](int64_t p) { return sid[p < n ? p : n - 1]; };         // (all asked for at once)
+  const int32_t before = c > 0 ? key(c * CHUNK - 1) : -1, last = key((c + 1) * CHUNK - 1), next = key((c + 1) * CHUNK);
+  const int32_t beyond = key((c + 1 + SHORT) * CHUNK);
+  const bool mine = lane < JOINERS && (c + 1) * CHUNK < n && last != NONE && next == last && before != last;
+  const bool far = mine && c + 1 + SHORT < chunks && beyond == last;
+  uint64_t longs = __ballot(far), near = __ballot(mine) & ~longs;
+  if (!(longs | near)) return;
   auto add_rows = [&](int64_t from, int64_t to, float s[VEC]) {        // part[k][0], from <= k < to
-    for (int64_t k = from; k < to; k += 16) {
-      float v[16][VEC];
+    constexpr int DEEP = 8;                                            // in flight together
+    for (int64_t k = from; k < to; k += DEEP) {
+      float v[DEEP][VEC];
 #pragma unroll
-      for (int q = 0; q < 16; ++q) load_cols<float, VEC>(part + ((k + q < to ? k + q : to - 1) * 2) * D + col, v[q]);
+      for (int q = 0; q < DEEP; ++q) load_cols<float, VEC>(part + ((k + q < to ? k + q : to - 1) * 2) * D + col, v[q]);
 #pragma unroll
-      for (int q = 0; q < 16; ++q)
+      for (int q = 0; q < DEEP; ++q)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s[e] = k + q < to ? s[e] + v[q][e] : s[e];
     }
   };
-  auto end_of = [&](int64_t first, int32_t id) {                       // the first chunk from `first` on that does not begin with id
-    for (int64_t step = 64; ; step = 1) {                              // by 64 at a time, then one by one
+  auto end_of = [&](int64_t first, int32_t id, int64_t step) {         // the first chunk from `first` on that does not begin with id
+    for (; ; step = 1) {                                               // by 64 at a time, then one by one
       while (true) {
         const int64_t k = first + (int64_t)lane * step;
         const uint64_t no = __ballot(!(k < chunks && sid[k * CHUNK] == id));
@@ -277,14 +335,13 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
       }
     }
   };
-  uint64_t near = todo & ~longs;
   for (int turn = 0; near; ++turn) {
     const int b = __ffsll((long long)near) - 1;
     near &= near - 1;
     if (turn % JOINERS != wave) continue;
-    const int64_t k = (int64_t)blockIdx.x * JOINERS + b;
-    const int32_t id = sid[(k + 1) * CHUNK - 1];
-    const int64_t end = end_of(k + 1, id);
+    const int64_t k = k0 + b;
+    const int32_t id = __shfl(last, b, 64);
+    const int64_t end = end_of(k + 1, id, 1);
     if (col < D) {
       float s[VEC];
       load_cols<float, VEC>(part + (k * 2 + 1) * D + col, s);
@@ -295,9 +352,9 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
   while (longs) {
     const int b = __ffsll((long long)longs) - 1;
     longs &= longs - 1;
-    const int64_t k = (int64_t)blockIdx.x * JOINERS + b;
-    const int32_t id = sid[(k + 1) * CHUNK - 1];
-    const int64_t end = end_of(k + 1, id), each = (end - (k + 1) + JOINERS - 1) / JOINERS;
+    const int64_t k = k0 + b;
+    const int32_t id = __shfl(last, b, 64);
+    const int64_t end = end_of(k + 1, id, 64), each = (end - (k + 1) + JOINERS - 1) / JOINERS;
     const int64_t from = k + 1 + wave * each, to = from + each < end ? from + each : end;
     float s[VEC];
 #pragma unroll
@@ -352,35 +409,29 @@ int launch_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, 
   uint32_t* pkey = (uint32_t*)(spos + n);
   int32_t* ppos = (int32_t*)pkey + (int64_t)np * PART;
   float* part = (float*)((char*)ws + list_bytes(n));
-  const int rankers = parts ? np : cdiv(n, 64);
-  const int64_t fills = accumulate ? 0 : ((int64_t)V * D + 4095) / 4096;
-  const int fillers = (int)(fills < 2048 ? fills : 2048);
   if (parts) {
     hipLaunchKernelGGL(part_sort_kernel, dim3(np), dim3(PART), 0, st, ids, ids64, n, V, pkey, ppos);
-    hipLaunchKernelGGL(order_kernel<true>, dim3(rankers + fillers), dim3(256), 0, st, ids, ids64, n, V, pkey, ppos, rankers, sid, spos, grad, V,
-                       D, ldg);
-  } else if (rankers + fillers) {
-    hipLaunchKernelGGL(order_kernel<false>, dim3(rankers + fillers), dim3(256), 0, st, ids, ids64, n, V, nullptr, nullptr, rankers, sid, spos,
-                       grad, V, D, ldg);
+    hipLaunchKernelGGL(order_kernel<true>, dim3(np), dim3(1024), 0, st, ids, ids64, n, V, pkey, ppos, sid, spos);
+  } else if (n > 0) {
+    hipLaunchKernelGGL(order_kernel<false>, dim3(cdiv(n, 64)), dim3(256), 0, st, ids, ids64, n, V, nullptr, nullptr, sid, spos);
   }
-  if (n > 0) {
-    const bool vec = D % 4 == 0 && aligned16(dy, lddy * 4) && (dy_f32 || lddy % 4 == 0) && aligned16(grad, ldg * 4);
-    const bool vec8 = vec && !dy_f32 && D % 8 == 0 && lddy % 8 == 0;                       // (16 bytes of a bf16 row per lane)
-    const int groups = cdiv(D, vec8 ? 512 : vec ? 256 : 64);
-    const int64_t chunks = (n + CHUNK - 1) / CHUNK, blocks = (chunks * groups + 3) / 4;
-    FDMI_CHECK(blocks < (1ll << 31), "embed_bwd: too many tokens");
-    const dim3 join((unsigned)((chunks + JOINERS - 1) / JOINERS), cdiv(D, vec ? 256 : 64));
+  const bool vec = D % 4 == 0 && aligned16(dy, lddy * 4) && (dy_f32 || lddy % 4 == 0) && aligned16(grad, ldg * 4);
+  const bool vec8 = vec && !dy_f32 && D % 8 == 0 && lddy % 8 == 0;                       // (16 bytes of a bf16 row per lane)
+  const int groups = cdiv(D, vec8 ? 512 : vec ? 256 : 64);
+  const int64_t chunks = (n + CHUNK - 1) / CHUNK, summers = chunks * groups, blocks = summers + (accumulate ? 0 : (V + ZROWS - 1) / ZROWS);
+  FDMI_CHECK(blocks < (1ll << 31), "embed_bwd: too many tokens");
+  if (blocks == 0) return 0;
+  const dim3 join((unsigned)((chunks + JOINERS - 1) / JOINERS), cdiv(D, vec ? 256 : 64));
 #define EMB_SUM(T, VEC) hipLaunchKernelGGL((run_sum_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)dy, lddy, sid, spos, n, D, \
-                                           groups, scale, accumulate, grad, ldg, part)
-    if (vec) {
-      if (dy_f32) EMB_SUM(float, 4); else if (vec8) EMB_SUM(bf16_t, 8); else EMB_SUM(bf16_t, 4);
-      hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
-    } else {
-      if (dy_f32) EMB_SUM(float, 1); else EMB_SUM(bf16_t, 1);
-      hipLaunchKernelGGL(run_join_kernel<1>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
-    }
-#undef EMB_SUM
+                                           groups, scale, accumulate, grad, ldg, part, (int)summers, V)
+  if (vec) {
+    if (dy_f32) EMB_SUM(float, 4); else if (vec8) EMB_SUM(bf16_t, 8); else EMB_SUM(bf16_t, 4);
+    if (chunks > 1) hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
+  } else {
+    if (dy_f32) EMB_SUM(float, 1); else EMB_SUM(bf16_t, 1);
+    if (chunks > 1) hipLaunchKernelGGL(run_join_kernel<1>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
   }
+#undef EMB_SUM
   FDMI_HIP(hipGetLastError());
   return 0;
 }

@@ -93,6 +93,46 @@ def test_gradient(n, V, D, kind, dt):
     assert torch.equal(got, again)                                     # a fixed order: the same bits
 
 
+# in the sorted list: runs that begin and end on, before and behind the edges of 16 and 64 positions, over one edge and over many
+RUNS = {"edges": [16, 48, 64, 1, 63, 65, 128, 15, 17, 31, 33, 2, 62, 64, 63, 1, 127, 129], "long": [7, 1100, 2, 1024, 64, 1089, 1, 4000, 63],
+        "whole": [64, 64, 64], "short": [1] * 200, "tail": [64, 1], "one more": [65]}
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("D", [5, 72, 520])
+@pytest.mark.parametrize("runs", list(RUNS))
+def test_gradient_of_runs_in_the_sorted_list(runs, D, dt):
+    ops = _ops()
+    lengths = RUNS[runs]
+    V = 2 * len(lengths) + 35                                          # every other row of the table has no token
+    ids = torch.cat([torch.full((k,), 2 * i + 1) for i, k in enumerate(lengths)])
+    g = torch.Generator().manual_seed(len(ids) + D)
+    ids = ids[torch.randperm(len(ids), generator=g)]
+    dy = _rand(len(ids), D, seed=7, dtype=dt)
+    v = _np(dy)
+    ref, mag, cnt = np.zeros((V, D)), np.zeros((V, D)), np.zeros((V, 1))
+    np.add.at(ref, ids.numpy(), v)
+    np.add.at(mag, ids.numpy(), np.abs(v))
+    np.add.at(cnt, ids.numpy(), 1.0)
+    full = torch.full((V, D), float("nan"), device="cuda")             # (the allocator hands its memory to the gradient)
+    del full
+    got = _np(ops.embed_bwd(dy.cuda(), ids.cuda(), V, scale=0.75))
+    assert (np.abs(got - 0.75 * ref) <= 0.75 * (cnt + 1) * 2.0 ** -24 * mag).all()      # (as above)
+    start = _rand(V, D, seed=8)
+    out = _np(ops.embed_bwd(dy.cuda(), ids.cuda(), V, scale=0.75, out=start.cuda()))
+    s = _np(start)
+    assert (np.abs(out - (s + 0.75 * ref)) <= (cnt + 2) * 2.0 ** -24 * (0.75 * mag + np.abs(s))).all()
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 2047, 2048, 2049, 2304])
+def test_gradient_where_the_order_is_found_another_way(n):
+    ops = _ops()
+    V, D = 150, 8
+    ids, dy = _ids_of("padded", n, V, n), _rand(n, D, seed=n).round()  # (integers: sums are exact)
+    ref = torch.zeros(V, D).index_add_(0, ids, dy)
+    assert torch.equal(ops.embed_bwd(dy.cuda(), ids.cuda(), V).cpu(), ref)
+
+
 def test_gradient_accumulates_into_strided_rows_and_leaves_the_others():
     ops = _ops()
     n, V, D = 200, 64, 70
