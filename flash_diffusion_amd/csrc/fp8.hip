@@ -254,36 +254,42 @@ __device__ __forceinline__ float act_of(int act, float v) {
   }
 }
 
-// eight consecutive columns of one row, with 16-byte accesses: the residual (16 bytes of bf16, 32 of fp32) ...
+// eight consecutive columns of one row, with 16-byte accesses at any address that an element may have (rows of odd lengths included: turned
+// round in LDS and stored by single columns, 4096 x 4100 x 4096 took 147 us): the residual (16 bytes of bf16, 32 of fp32) ...
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <bool F32>
 __device__ __forceinline__ void load_res8(const Fp8GemmArgs& a, int m, int n, uint4 r[F32 ? 2 : 1]) {
-  if constexpr (F32) {
-    const uint4* p = (const uint4*)((const float*)a.residual + (int64_t)m * a.ldr + n);
-    r[0] = p[0];
-    r[1] = p[1];
-  } else {
-    r[0] = *(const uint4*)((const bf16_t*)a.residual + (int64_t)m * a.ldr + n);
+  const char* p = (const char*)a.residual + ((int64_t)m * a.ldr + n) * (F32 ? 4 : 2);
+#pragma unroll
+  for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+    const u32x4_any t = *(const u32x4_any*)(p + 16 * i);
+    r[i] = make_uint4(t[0], t[1], t[2], t[3]);
   }
 }
-// ... and sums + bias, activation, + residual, stored.  Rows of C, the residual and the bias are aligned
+// ... and sums + bias, activation, + residual, stored
 template <bool F32>
 __device__ __forceinline__ void store8(const Fp8GemmArgs& a, int m, int n, float v[8], const uint4 r[F32 ? 2 : 1]) {
   if (a.bias) {
-    const float4 p = *(const float4*)(a.bias + n), q = *(const float4*)(a.bias + n + 4);
-    v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w; v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
+    const f32x4_any p = *(const f32x4_any*)(a.bias + n), q = *(const f32x4_any*)(a.bias + n + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] += p[i];
+      v[4 + i] += q[i];
+    }
   }
   if (a.act) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = act_of(a.act, v[i]);
   }
   if constexpr (F32) {
-    float* c = (float*)a.C + (int64_t)m * a.ldc + n;
     if (a.residual) {
       v[0] += __uint_as_float(r[0].x); v[1] += __uint_as_float(r[0].y); v[2] += __uint_as_float(r[0].z); v[3] += __uint_as_float(r[0].w);
       v[4] += __uint_as_float(r[1].x); v[5] += __uint_as_float(r[1].y); v[6] += __uint_as_float(r[1].z); v[7] += __uint_as_float(r[1].w);
     }
-    *(float4*)c = make_float4(v[0], v[1], v[2], v[3]);
-    *(float4*)(c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    float* c = (float*)a.C + (int64_t)m * a.ldc + n;
+    *(f32x4_any*)c = (f32x4_any){v[0], v[1], v[2], v[3]};
+    *(f32x4_any*)(c + 4) = (f32x4_any){v[4], v[5], v[6], v[7]};
   } else {
     if (a.residual) {
       const uint32_t t[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
@@ -293,7 +299,7 @@ __device__ __forceinline__ void store8(const Fp8GemmArgs& a, int m, int n, float
         v[2 * i + 1] += __uint_as_float(t[i] & 0xffff0000u);
       }
     }
-    *(uint4*)((bf16_t*)a.C + (int64_t)m * a.ldc + n) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+    *(u32x4_any*)((bf16_t*)a.C + (int64_t)m * a.ldc + n) = (u32x4_any){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
   }
 }
 __device__ __forceinline__ void store1(const Fp8GemmArgs& a, int m, int n, float v) {
@@ -325,20 +331,20 @@ constexpr int BAND = 4;                                               // tile ro
 constexpr int SEG = 48;                                              // blocks of 128 per item
 constexpr int fp8_segments(int kb) { return (kb + SEG - 1) / SEG; }
 constexpr int fp8_segment(int kb) { return (kb + fp8_segments(kb) - 1) / fp8_segments(kb); }
-// LDS: the ring, two panels of scales ([block][BM rows of X | 8 groups of W]; the last transfer into one may be whole), and what the
-// epilogue needs: a row of the gated form's maxima per wave column, or 32 x (32 NF + 1) floats per wave to turn ragged tiles round
+// LDS: the ring, two panels of scales ([block][BM rows of X | 8 groups of W]; the last transfer into one may be whole), and the
+// gated form's maxima, one per row and wave column
 constexpr int fp8_panel(int BM, int kb) { return (kb < SEG ? kb : SEG) * (BM + 8) + 256; }
-constexpr int fp8_smem(int BM, int BN, int WM, int WN, bool gated, bool vec, int kb) {
-  return 4 * (BM + BN) * 64 + 2 * fp8_panel(BM, kb) + (gated ? BM * WN * 4 : vec ? 0 : WM * WN * 32 * (BN / WN + 1) * 4);
+constexpr int fp8_smem(int BM, int BN, int WM, int WN, bool gated, int kb) {
+  return 4 * (BM + BN) * 64 + 2 * fp8_panel(BM, kb) + (gated ? BM * WN * 4 : 0);
 }
 
-template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE, bool VEC>
-__global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArgs a, int tilesM, int tilesN) {
+template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE>
+__global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(const Fp8GemmArgs a, int row0, int tilesM, int tilesN) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NW = WM * WN, MF = BM / WM / 32, NF = BN / WN / 32, STAGE = (BM + BN) * 64;
   constexpr int AP = BM / 16 / NW, WP = BN / 16 / NW, PIECES = AP + WP;   // 1 KiB pieces (16 rows) per wave and stage
   constexpr int AHEAD = MF >= 2 ? 2 : 1, RING = 2 * MF >= 4 ? 4 : 2, BURST = (PIECES + MF - 1) / MF, LATE = AHEAD * BURST < PIECES ? AHEAD * BURST : PIECES;
-  static_assert(AP >= 1 && WP >= 1 && NW % 4 == 0 && (!GATED || (NF == 2 && BN == 256 && VEC)), "tile shape");
+  static_assert(AP >= 1 && WP >= 1 && NW % 4 == 0 && (!GATED || (NF == 2 && BN == 256)), "tile shape");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN, half = lane >> 5, j = lane & 31;
   const int total = tilesM * tilesN, G = gridDim.x;
@@ -353,7 +359,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
     const int xcd = it.v & 7, qd = total >> 3, rem = total & 7;
     const int t = (xcd < rem ? xcd * (qd + 1) : rem * (qd + 1) + (xcd - rem) * qd) + (it.v >> 3);
     const int band = t / (BAND * tilesN), in = t - band * BAND * tilesN, rows = tilesM - band * BAND < BAND ? tilesM - band * BAND : BAND;
-    it.m0 = (band * BAND + in % rows) * BM;
+    it.m0 = row0 + (band * BAND + in % rows) * BM;
     it.n0 = (in / rows) * BN;
     it.mt = it.m0 >> 4;
     if (it.mt > Mt - BM / 16) it.mt = Mt > BM / 16 ? Mt - BM / 16 : 0;
@@ -486,7 +492,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
         }
       }
       __syncthreads();                                                // (red is written again by the next tile)
-    } else if constexpr (VEC) {
+    } else {
       // lanes l and l + 32 hold alternating runs of four columns: exchange so that each has eight consecutive ones.  The residual of the next
       // 32 rows is asked for before these are stored (C may be the residual, so the compiler keeps loads behind the stores before them;
       // 8192^3 with a residual: 457 us without, 441 with the loads ahead)
@@ -498,7 +504,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int n = nw + i * 32 + r * 16 + half * 8;
-            if (m >= it.m0 && m < a.M && n < a.N) load_res8<WIDE>(a, m, n, res[k & 1][i][r]);
+            if (m >= it.m0 && m < a.M && n + 8 <= a.N) load_res8<WIDE>(a, m, n, res[k & 1][i][r]);
           }
       };
       if (a.residual) fetch(0);
@@ -519,23 +525,18 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(const Fp8GemmArg
               v[4 + t] = __uint_as_float(e[1]);
             }
             const int n = nw + i * 32 + r * 16 + half * 8;
-            if (m >= it.m0 && m < a.M && n < a.N) store8<WIDE>(a, m, n, v, res[k & 1][i][r]);
+            if (m >= it.m0 && m < a.M) {
+              if (n + 8 <= a.N) store8<WIDE>(a, m, n, v, res[k & 1][i][r]);
+              else {                                                  // the last columns of a row, one by one (unrolled, the 256 x 256
+#pragma unroll 1                                                      // tile spills over it: 16384 x 10240 x 4096 in 597 us instead of 526)
+                for (int c = n; c < a.N; ++c) {
+                  store1(a, m, c, v[0]);
+#pragma unroll
+                  for (int t = 0; t < 7; ++t) v[t] = v[t + 1];
+                }
+              }
+            }
           }
-      }
-    } else {
-      // rows of C that are not aligned: each wave turns 32 rows at a time round in LDS and stores single columns
-      constexpr int LD = NF * 32 + 1;
-      float* turn = (float*)(smem + 4 * STAGE + 2 * panel_bytes) + wave * 32 * LD;
-#pragma unroll
-      for (int k = 0; k < MF; ++k) {
-#pragma unroll
-        for (int i = 0; i < NF; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) turn[j * LD + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3)] = acc[i][k][r];
-        for (int e = lane; e < 32 * NF * 32; e += 64) {
-          const int m = mw + k * 32 + e / (NF * 32), n = nw + e % (NF * 32);
-          if (m >= it.m0 && m < a.M && n < a.N) store1(a, m, n, turn[e / (NF * 32) * LD + e % (NF * 32)]);
-        }
       }
     }
 #pragma unroll
@@ -638,21 +639,22 @@ int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
   return 0;
 }
 
-template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE, bool VEC>
-int launch_tile(const Fp8GemmArgs& a, hipStream_t st) {
-  constexpr int most = fp8_smem(BM, BN, WM, WN, GATED, VEC, SEG);
+// the rows from row0 on (a multiple of 16), `rows` of them (a multiple of BM, or all)
+template <int BM, int BN, int WM, int WN, bool GATED, bool WIDE>
+int launch_tile(const Fp8GemmArgs& a, hipStream_t st, int row0 = 0, int rows = 0) {
+  constexpr int most = fp8_smem(BM, BN, WM, WN, GATED, SEG);
   static_assert(most <= 160 * 1024, "LDS");
   static std::atomic<uint64_t> allowed;
-  if (const int rc = allow_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE, VEC>, most, allowed)) return rc;
-  const int smem = fp8_smem(BM, BN, WM, WN, GATED, VEC, a.Kb);
-  const int64_t tilesM = ((int64_t)a.M + BM - 1) / BM, tilesN = ((int64_t)a.N * (GATED ? 2 : 1) + BN - 1) / BN;
+  if (const int rc = allow_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>, most, allowed)) return rc;
+  const int smem = fp8_smem(BM, BN, WM, WN, GATED, a.Kb);
+  const int64_t tilesM = ((int64_t)(rows ? rows : a.M - row0) + BM - 1) / BM, tilesN = ((int64_t)a.N * (GATED ? 2 : 1) + BN - 1) / BN;
   FDMI_CHECK(tilesM * tilesN < (1ll << 30), "gemm_fp8: too many tiles");
   // as many workgroups as fit (a multiple of the 8 XCDs); one per tile where an item is too short for the ring to run across items
   int fit = 160 * 1024 / smem;
   if (fit > 2048 / (WM * WN * 64)) fit = 2048 / (WM * WN * 64);
   const int64_t room = (int64_t)256 * fit, total = tilesM * tilesN;
   const int64_t grid = a.Kb < 2 || total < room ? total : room;
-  hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE, VEC>), dim3((unsigned)grid), dim3(WM * WN * 64), smem, st, a, (int)tilesM,
+  hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>), dim3((unsigned)grid), dim3(WM * WN * 64), smem, st, a, row0, (int)tilesM,
                      (int)tilesN);
   FDMI_HIP(hipGetLastError());
   return 0;
@@ -821,22 +823,30 @@ int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t
   return 0;
 }
 
-// Which kernel: the least of the times measured for each, as a function of the problem (microseconds).  A tile kernel spends `block` + `share` * w
-// on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU rounded up; the streaming kernel is bound by what its workgroups
-// read from L2 (25 TB/s over all CUs; a short grid leaves some idle) or by the weight from memory.  Measured against each other at
-// 8192^3, 1920 x 4096 x {4096, 10240}, {1, 16, 64} x 4096 x 4096, 512 x 1024 x 4096, 120 x 1024 x 2560, 2048 x 2048 x 4096, for example
-// (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 15.7 / 22.8 / 36, 4.3;  1920 x 4096 x 4096: 58 / 32.6 / 32.2 / 46, 72;
-// 1920 x 10240 x 4096: 122 / 73.2 / 80.0 / 89, 246;  8192^3: 1002 / 445 / 437 / 381, 2266;  16384 x 10240 x 4096: 1382 / 603 / 582 / 503, 2018.
-struct Fp8Cost { int BM, BN; double block, share, fixed, tile; };
-double fp8_cost(const Fp8GemmArgs& a, const Fp8Cost& c) {
-  const double tiles = double((a.M + c.BM - 1) / c.BM) * ((a.N + c.BN - 1) / c.BN), w = (double)(int64_t)((tiles + 255) / 256);
-  return c.fixed + c.tile * w + a.Kb * (c.block + c.share * w);
+// Which kernel: the least of the times that formulas in the problem's sizes give (microseconds), their constants fitted to times of every kernel on 148
+// problems (16 .. 16384 rows, 64 .. 12288 columns, K 64 .. 10240; half of them drawn, half large).  The chosen one is 4% slower than
+// the best on average (at most 1.6 times, where both are below 3 us).  A tile kernel spends `block` + `share` * w on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU
+// rounded up; a grid that leaves CUs idle runs its blocks up to `idle` faster.  The streaming kernel is bound by what its workgroups read
+// from L2 (a short grid leaves some CUs idle) or by the weight from memory, and pays for each further turn of 1024 workgroups.
+// For example (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 15.7 / 22.8 / 36, 4.3;  1920 x 4096 x 4096:
+// 57 / 33.6 / 32.9 / 47, 86;  1920 x 10240 x 4096: 123 / 75.5 / 83.9 / 93, 246;  8192^3: 935 / 469 / 477 / 403, 2234.
+struct Fp8Cost { int BM, BN; double block, share, fixed, tile, idle; };
+double fp8_cost(int64_t M, int64_t N, int Kb, const Fp8Cost& c) {
+  const double tiles = double((M + c.BM - 1) / c.BM) * ((N + c.BN - 1) / c.BN), w = (double)(int64_t)((tiles + 255) / 256);
+  return c.fixed + c.tile * w + Kb * (c.block + c.share * w * (tiles < 256 ? 1. - c.idle * (1. - tiles / 256) : 1.));
 }
 double fp8_stream_cost(const Fp8GemmArgs& a, int rows) {   // `rows` rows of X and of W per workgroup
-  double groups = double((a.M + rows - 1) / rows) * ((a.N + rows - 1) / rows);
-  if (groups < 256) groups = 256;
-  const double l2 = groups * 2 * rows * a.Kb * 128 / 25e6, hbm = double(a.N) * a.Kb * 128 / 4.5e6;
-  return 2.7 + (l2 > hbm ? l2 : hbm);
+  const double groups = double((a.M + rows - 1) / rows) * ((a.N + rows - 1) / rows), more = (double)(int64_t)((groups - 1) / 1024);
+  const double l2 = (groups < 256 ? 256 : groups) * 2 * rows * a.Kb * 128 / 24e6, hbm = double(a.N) * a.Kb * 128 / 4.5e6;
+  return (rows == 16 ? 3.5 + .5 * more : 3. + 1.3 * more) + (l2 > hbm ? l2 : hbm);
+}
+constexpr double FP8_LAUNCH = 1.5;                         // a second launch on the same stream
+// The largest tiles are the fastest per product and leave the most CUs idle in the last turn.  The rows that fill whole turns of 256 x 256
+// tiles; the others may go to a second launch of smaller ones (gated 1920 x 4096 -> 10240: 153 us on 128-row tiles, 111 + 33 on 1536 rows of the
+// large and 384 of the small; 3500 x 5120 x 2048: 49 us)
+int fp8_whole(int64_t M, int64_t N) {
+  const int64_t cols = (N + 255) / 256, turns = M / 256 * cols / 256;
+  return (int)(turns * 256 / cols * 256);
 }
 
 // whether a product of unquantised rows quantises them inside the streaming kernel
@@ -848,28 +858,53 @@ int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st) {
     if (a.x_f32) return a.out_f32 ? launch_stream<1, 1, true, float>(a, st) : launch_stream<1, 1, false, float>(a, st);
     return a.out_f32 ? launch_stream<1, 1, true, bf16_t>(a, st) : launch_stream<1, 1, false, bf16_t>(a, st);
   }
-  if (a.H) return ((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 128 ? launch_tile<64, 256, 1, 4, true, false, true>(a, st) : launch_tile<128, 256, 2, 4, true, false, true>(a, st);
-  const int es = a.out_f32 ? 4 : 2;
-  const bool vec = a.N % 8 == 0 && aligned(a.C, a.ldc * es, 16) && (!a.residual || aligned(a.residual, a.ldr * es, 16)) && ((uintptr_t)a.bias & 15) == 0;
-  static const Fp8Cost narrow[] = {{64, 64, .09, .172, 3., .5}, {128, 128, .02, .46, 3., 1.}, {128, 256, 0., .86, 3., 3.}, {256, 256, 0., 1.45, 3., 5.}};
-  static const Fp8Cost wide[] = {{64, 64, .20, .25, 3., .5}, {128, 128, .13, .80, 3., 1.}, {256, 256, 0., 3., 3., 5.}};
-  const Fp8Cost* table = a.out_f32 ? wide : narrow;
-  int best = -1;
-  double least = 0.;
-  for (int i = 0; i < (a.out_f32 ? 3 : 4); ++i) {
-    if (table[i].BN > 128 && !vec) continue;               // (no room in LDS to turn ragged tiles round)
-    const double c = fp8_cost(a, table[i]);
-    if (best < 0 || c < least) { best = i; least = c; }
+  static const Fp8Cost narrow[] = {{64, 64, .08, .174, 2.4, .63, 0.}, {128, 128, .06, .384, 3.3, 1.8, .27}, {128, 256, .07, .744, .9, 4.3, .34},
+                                   {256, 256, .10, 1.39, .2, 7.5, .39}};
+  static const Fp8Cost wide[] = {{64, 64, .20, .265, 2., .95, 0.}, {128, 128, .27, .69, 2., 3.25, .37}, {256, 256, .33, 2.74, 0., 9.8, .43}};
+  if (a.H) {
+    const int64_t cols = ((int64_t)a.N + 127) / 128 * 256;
+    if (((int64_t)a.M + 127) / 128 * (cols / 256) < 128) return launch_tile<64, 256, 1, 4, true, false>(a, st);
+    const int whole = fp8_whole(a.M, cols), rest = a.M - whole;
+    const double small = fp8_cost(a.M, cols, a.Kb, narrow[2]), large = fp8_cost(a.M, cols, a.Kb, narrow[3]);
+    const double both = whole && rest ? fp8_cost(whole, cols, a.Kb, narrow[3]) + FP8_LAUNCH + fp8_cost(rest, cols, a.Kb, narrow[2]) : 1e30;
+    if (small <= large && small <= both) return launch_tile<128, 256, 2, 4, true, false>(a, st);
+    if (large <= both) return launch_tile<256, 256, 2, 4, true, false>(a, st);
+    if (const int rc = launch_tile<256, 256, 2, 4, true, false>(a, st, 0, whole)) return rc;
+    return launch_tile<128, 256, 2, 4, true, false>(a, st, whole);
   }
+  const Fp8Cost* table = a.out_f32 ? wide : narrow;
+  const int kinds = a.out_f32 ? 3 : 4;
+  auto cheapest = [&](int64_t rows, double& least) {
+    int best = -1;
+    for (int i = 0; i < kinds; ++i) {
+      const double c = fp8_cost(rows, a.N, a.Kb, table[i]);
+      if (best < 0 || c < least) { best = i; least = c; }
+    }
+    return best;
+  };
+#define FP8_TILE(BM, BN, WM, WN, WIDE) launch_tile<BM, BN, WM, WN, false, WIDE>(a, st, row0, rows)
+  auto run = [&](int kind, int row0, int rows) {
+    switch (table[kind].BM + table[kind].BN) {
+      case 128: return a.out_f32 ? FP8_TILE(64, 64, 2, 2, true) : FP8_TILE(64, 64, 2, 2, false);
+      case 256: return a.out_f32 ? FP8_TILE(128, 128, 2, 2, true) : FP8_TILE(128, 128, 2, 2, false);
+      case 384: return FP8_TILE(128, 256, 2, 4, false);
+      default:
+        return a.out_f32 ? FP8_TILE(256, 256, 2, 4, true) : FP8_TILE(256, 256, 2, 4, false);
+    }
+  };
+#undef FP8_TILE
+  double least = 0., tail = 0.;
+  const int best = cheapest(a.M, least);
   const double s16 = fp8_stream_cost(a, 16), s32 = fp8_stream_cost(a, 32);
   if (s16 <= s32 && s16 < least) return a.out_f32 ? launch_stream<1, 1, true, void>(a, st) : launch_stream<1, 1, false, void>(a, st);
   if (s32 < least) return a.out_f32 ? launch_stream<2, 2, true, void>(a, st) : launch_stream<2, 2, false, void>(a, st);
-#define FP8_TILE(BM, BN, WM, WN, WIDE) (vec ? launch_tile<BM, BN, WM, WN, false, WIDE, true>(a, st) : launch_tile<BM, BN, WM, WN, false, WIDE, false>(a, st))
-  switch (table[best].BM + table[best].BN) {
-    case 128: return a.out_f32 ? FP8_TILE(64, 64, 2, 2, true) : FP8_TILE(64, 64, 2, 2, false);
-    case 256: return a.out_f32 ? FP8_TILE(128, 128, 2, 2, true) : FP8_TILE(128, 128, 2, 2, false);
-    case 384: return launch_tile<128, 256, 2, 4, false, false, true>(a, st);
-    default: return a.out_f32 ? launch_tile<256, 256, 2, 4, false, true, true>(a, st) : launch_tile<256, 256, 2, 4, false, false, true>(a, st);
+  const int whole = fp8_whole(a.M, a.N);
+  if (whole && whole < a.M) {
+    const int kind = cheapest(a.M - whole, tail);
+    if (kind != kinds - 1 && fp8_cost(whole, a.N, a.Kb, table[kinds - 1]) + FP8_LAUNCH + tail < least) {
+      if (const int rc = run(kinds - 1, 0, whole)) return rc;
+      return run(kind, whole, 0);
+    }
   }
-#undef FP8_TILE
+  return run(best, 0, 0);
 }

@@ -268,6 +268,69 @@ def test_the_gated_feed_forward_as_a_whole():
     assert off <= 0.1 * 2.0 ** -4 * np.linalg.norm(f) + 2.0 ** -8 * np.linalg.norm(f + v)
 
 
+# ---- large products: tiles of every size, several of them per workgroup, contractions in segments, rows in two launches ----------------------
+def _pipe64(x, w):
+    """R.pipe_bound on the GPU"""
+    g = lambda t: torch.nn.functional.pad(t, (0, -t.shape[1] % 8)).abs().reshape(t.shape[0], -1, 8).amax(2)
+    return 2.0 ** -10 * (g(x) @ g(w).t().contiguous())
+
+
+def _operands64(M, N, K, seed):
+    ops = _ops()
+    x, w = _rand(M, K, seed=seed, dtype=BF16, spread=1.0).cuda(), (_rand(N, K, seed=seed + 1) * K ** -0.5).cuda()
+    q, W = ops.quant_fp8(x), ops.pack_weight_fp8(w)                    # (compared with the plain format above)
+    return q, W, q.values(F32).double(), W.values(F32).double()
+
+
+LARGE = [(1920, 4096, 520), (1930, 2568, 6300), (4096, 4096, 6272), (2048, 2051, 1300), (3500, 5120, 2048), (5000, 1800, 1030), (700, 6152, 385),
+         (4360, 2176, 200)]
+
+
+@pytest.mark.parametrize("yt", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", LARGE)
+def test_large_product(M, N, K, yt):
+    ops = _ops()
+    q, W, xv, wv = _operands64(M, N, K, M + N)
+    b, r = _rand(N, seed=3).cuda(), _rand(M, N, seed=4, dtype=yt).cuda()
+    ref, mag = xv @ wv.t().contiguous(), xv.abs() @ wv.abs().t().contiguous()
+    pipe = _pipe64(xv, wv) if yt == BF16 else 0.0
+    for bias, res in ((None, None), (b, r)):
+        want = ref if bias is None else ref + b.double() + r.double()
+        add = 0.0 if bias is None else b.double().abs() + r.double().abs()
+        e = R.sum_bound(K + 4) * (mag + add) + pipe                   # (as in _check)
+        tol = e + R.half_step(NAMES[yt]) * (want.abs() + e)
+        d = (ops.gemm_fp8(q, W, bias=bias, residual=res, out_f32=yt == F32).double() - want).abs()
+        assert bool((d <= tol).all()), (float((d - tol).max()), float(d.max()))
+    out = r.clone()                                                   # the result over its own residual
+    assert torch.equal(ops.gemm_fp8(q, W, bias=b, residual=out, out=out), ops.gemm_fp8(q, W, bias=b, residual=r, out_f32=yt == F32))
+
+
+@pytest.mark.parametrize("M,N,K", [(3500, 2560, 2048), (2048, 4096, 384), (1100, 2600, 300), (1920, 1300, 6272)])
+def test_large_gated_product(M, N, K):
+    ops = _ops()
+    q, W0, xv, v0 = _operands64(M, N, K, 5)
+    W1 = ops.pack_weight_fp8((_rand(N, K, seed=9) * K ** -0.5).cuda())
+    v1 = W1.values(F32).double()
+    h = ops.gated_fp8(q, W0, W1)
+    t = lambda w: w.t().contiguous()
+    a, b, ax = xv @ t(v0), xv @ t(v1), xv.abs()
+    gelu = torch.nn.functional.gelu(a, approximate="tanh")
+    ref = gelu * b
+    # (as in test_gated_product)
+    ea, eb = R.sum_bound(K) * (ax @ t(v0.abs())) + _pipe64(xv, v0), R.sum_bound(K) * (ax @ t(v1.abs())) + _pipe64(xv, v1)
+    e = 1.2 * ea * (b.abs() + eb) + (gelu.abs() + 2e-6) * eb + 2e-6 * (1 + a.abs()) * b.abs()
+    nb = -(-N // 128)
+    s = torch.from_numpy(_exps(h)).cuda()
+    pad = lambda u: torch.nn.functional.pad(u, (0, nb * 128 - N)).reshape(M, nb, 128).amax(2)
+    sc = torch.pow(2.0, s.double())
+    assert bool((pad((ref.abs() - e).clamp_min(0)) <= 448.0 * sc).all())
+    assert bool(((pad(ref.abs() + e) > 224.0 * sc) | (s == -127)).all())
+    full = sc.repeat_interleave(128, 1)[:, :N]
+    d = (h.values(F32).double() - ref).abs()
+    tol = torch.maximum(2.0 ** -4 * (ref.abs() + e), 2.0 ** -10 * full) + e
+    assert bool((d <= tol).all()), float((d - tol).max())
+
+
 def test_two_runs_are_bit_identical_and_a_graph_replays_them():
     ops = _ops()
     M, N, K = 200, 300, 520
