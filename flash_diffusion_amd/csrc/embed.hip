@@ -77,7 +77,9 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t 
 // one by one (quadratic, but one launch: 4.6 us at 256 positions, 7.4 at 1232, 10.1 at 2048, 18 at 4096, 58 at 16384).  Longer lists are
 // first sorted in parts of 256; the other parts' counts are then binary searches (two launches: 9.1 us at 1232, 9.2 at 2048, 9.7 at 4096,
 // 17.5 at 16384, 98 at 131072; between two launches lies a microsecond).
-constexpr int DIRECT = 2048, PART = 256;
+// Each part is searched by every other one, so a call of more than SLICE positions (as many parts as run at once) adds up slice after slice:
+// 2^20 positions of 512 bf16 columns take 1.2 ms (as one list the order alone would: 92 us at 2^17, and it grows with the square).
+constexpr int DIRECT = 2048, PART = 256, SLICE = 512 * PART;
 constexpr int TILE = 4096;             // keys in LDS at a time
 
 __device__ __forceinline__ uint32_t key_of(const void* ids, int ids64, int64_t V, int64_t p) {
@@ -399,8 +401,11 @@ int launch_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t
 
 // scratch: the sorted list's keys and positions, those of the sorted parts, and two partial rows per chunk
 static int64_t list_bytes(int64_t n) { return ((n > DIRECT ? n + (n + PART - 1) / PART * PART : n) * 2 * 4 + 255) / 256 * 256; }
-int64_t embed_bwd_ws_bytes(int64_t n, int D) { return list_bytes(n) + (n + CHUNK - 1) / CHUNK * 2 * (int64_t)D * 4; }
-int launch_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
+int64_t embed_bwd_ws_bytes(int64_t n, int D) {
+  if (n > SLICE) n = SLICE;
+  return list_bytes(n) + (n + CHUNK - 1) / CHUNK * 2 * (int64_t)D * 4;
+}
+static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
                      int accumulate, float* grad, int64_t ldg, void* ws, hipStream_t st) {
   const bool parts = n > DIRECT;
   const int np = cdiv(n, PART);
@@ -433,5 +438,17 @@ int launch_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, 
   }
 #undef EMB_SUM
   FDMI_HIP(hipGetLastError());
+  return 0;
+}
+
+int launch_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
+                     int accumulate, float* grad, int64_t ldg, void* ws, hipStream_t st) {
+  int64_t at = 0;
+  do {
+    const int64_t now = n - at < SLICE ? n - at : SLICE;
+    if (const int rc = launch_slice((const char*)dy + at * lddy * (dy_f32 ? 4 : 2), dy_f32, lddy, (const char*)ids + at * (ids64 ? 8 : 4), ids64, now, V, D,
+                                    scale, accumulate || at > 0, grad, ldg, ws, st)) return rc;
+    at += now;
+  } while (at < n);
   return 0;
 }

@@ -133,6 +133,33 @@ def test_gradient_where_the_order_is_found_another_way(n):
     assert torch.equal(ops.embed_bwd(dy.cuda(), ids.cuda(), V).cpu(), ref)
 
 
+@pytest.mark.parametrize("n,it", [(131073, torch.int32), (300000, torch.int64)])
+def test_gradient_of_long_lists(n, it):
+    ops = _ops()
+    V, D = 700, 12
+    ids, dy = _ids_of("padded", n, V, n), torch.randint(-3, 4, (n, D), generator=torch.Generator().manual_seed(n))
+    ref = torch.zeros(V, D, dtype=torch.int64).index_add_(0, ids, dy).float()
+    for dt in (F32, BF16):                                             # (integers below 2^24: sums are exact)
+        assert torch.equal(ops.embed_bwd(dy.to(dt).cuda(), ids.to(it).cuda(), V).cpu(), ref)
+        out = torch.ones(V, D, device="cuda")
+        assert torch.equal(ops.embed_bwd(dy.to(dt).cuda(), ids.to(it).cuda(), V, out=out).cpu(), ref + 1)
+
+
+def test_tables_beyond_two_to_the_31_elements():
+    ops = _ops()
+    V, D = 540000, 4096
+    ids = torch.tensor([[0, V - 1, V - 2], [524287, 524288, 524289]], device="cuda")
+    table = torch.zeros(V, D, dtype=BF16, device="cuda")
+    rows = _rand(6, D, dtype=BF16).cuda()
+    table[ids.view(-1)] = rows
+    assert torch.equal(ops.embed_fwd(table, ids).view(6, D), rows)
+    del table
+    g = ops.embed_bwd(rows.view(2, 3, D), ids, V)
+    assert torch.equal(g[ids.view(-1)], rows.float())
+    g[ids.view(-1)] = 0.0
+    assert not g.any()
+
+
 def test_gradient_accumulates_into_strided_rows_and_leaves_the_others():
     ops = _ops()
     n, V, D = 200, 64, 70
