@@ -457,7 +457,7 @@ bool fp8_ok(const void* codes, const void* scales, int64_t K) {
 
 int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, void* codes, void* scales, int64_t M, int K,
                    void* stream) {
-  FDMI_CHECK(M >= 0 && M < (1ll << 31) && K >= 1, "quant_fp8: need M >= 0 and K >= 1");
+  FDMI_CHECK(M >= 0 && M <= (1ll << 30) && K >= 1, "quant_fp8: need 0 <= M <= 2^30 and K >= 1");
   if (M == 0) return 0;
   FDMI_CHECK(x && ldx >= K, "quant_fp8: x rows shorter than K");
   FDMI_CHECK(fp8_ok(codes, scales, K), "quant_fp8: codes are 16-byte, scales 4-byte aligned, K <= 131072");
@@ -471,7 +471,7 @@ int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* cod
   return launch_pack_fp8(w, w_f32, ldw, N, K, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)codes_t, (uint8_t*)scales_t, (hipStream_t)stream);
 }
 int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
-  FDMI_CHECK(d && d->M >= 0 && d->N >= 1 && d->K >= 1, "gemm_fp8: need M >= 0, N >= 1, K >= 1");
+  FDMI_CHECK(d && d->M >= 0 && d->M <= (1 << 30) && d->N >= 1 && d->N <= (1 << 17) && d->K >= 1, "gemm_fp8: need 0 <= M <= 2^30, 1 <= N <= 131072, K >= 1");
   if (d->M == 0) return 0;
   const bool fused = d->x && !d->W2 && fp8_fused(d->M, d->K);
   FDMI_CHECK((fused || fp8_ok(d->X, d->sx, d->K)) && fp8_ok(d->W, d->sw, d->K), "gemm_fp8: codes are 16-byte, scales 4-byte aligned, K <= 131072");

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -16,8 +17,9 @@ BF16, F32 = torch.bfloat16, torch.float32
 
 class PackedFp8:
     """The 8-bit form of ONE parameter, packed on first use and again when the parameter has changed (replaced, moved, or written in place:
-    torch counts those).  The parameter itself is held, so another one at the same address is not taken for it.  Streams other than
-    the one it was packed on wait for the packing; a capture cannot pack (run the layer once before)."""
+    torch counts those, but for writes through .data).  It is packed again into the same memory where shape and device allow, so a
+    captured graph that reads it sees the new weight.  The parameter itself is held, so another one at the same address is not taken
+    for it.  Streams other than the one it was packed on wait for the packing; a capture cannot pack (run the layer once before)."""
 
     def __init__(self, transposed=False):
         self.transposed = transposed
@@ -35,9 +37,12 @@ class PackedFp8:
         if self._of is not w or self._key != key:
             if capturing:
                 raise RuntimeError("the weight has to be packed before a graph is captured: run the layer once")
-            if self._packed is not None:
-                torch.cuda.synchronize()           # (a stream may still read the codes that are dropped here)
-            packed, stream, event = ops.pack_weight_fp8(w.detach().contiguous(), self.transposed), torch.cuda.current_stream(), torch.cuda.Event()
+            old, into = self._packed, None
+            if old is not None:
+                torch.cuda.synchronize()           # (a stream may still read the codes that are overwritten or dropped here)
+                into = old if (old.N, old.K, old.codes.device) == (*w.shape, w.device) else None
+            packed = ops.pack_weight_fp8(w.detach().contiguous(), self.transposed, into)
+            stream, event = torch.cuda.current_stream(), torch.cuda.Event()
             event.record(stream)
             self._packed, self._stream, self._event = packed, stream, event
             self._key, self._of = key, w
@@ -57,6 +62,7 @@ class _Fp8LinearFn(torch.autograd.Function):
         return y.view(*x.shape[:-1], packed.N)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dy = dy.reshape(-1, dy.shape[-1])
         if dy.shape[1] > 1 and dy.stride(1) != 1 or dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]:
@@ -104,6 +110,7 @@ class _LookupFn(torch.autograd.Function):
         return ops.embed_fwd(weight, ids, scale=scale, pos=pos, dtype=dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         dy = dy.contiguous()

@@ -2,6 +2,7 @@
 memory and the current stream; every computation below runs in a hand-written HIP kernel."""
 from __future__ import annotations
 
+import copy
 import ctypes as C
 
 import torch
@@ -446,6 +447,22 @@ def _rows(t, what, dtypes=(BF16, F32)):
     return ld
 
 
+def _overlap(a, b):
+    """whether two 2-D operands with contiguous rows (as _rows accepts them) share memory: False for disjoint ranges and for disjoint
+    columns of rows of one stride"""
+    def span(t):
+        es, (M, K) = t.element_size(), t.shape
+        ld = t.stride(0) * es if M > 1 else K * es
+        return t.data_ptr(), (M - 1) * ld + K * es, ld, K * es
+    if not a.numel() or not b.numel():
+        return False
+    (pa, na, la, wa), (pb, nb, lb, wb) = span(a), span(b)
+    if pa + na <= pb or pb + nb <= pa:
+        return False
+    d = (pb - pa) % la
+    return not (la == lb and d >= wa and d + wb <= la)
+
+
 def _vector(t, n, what):
     _here(t, what)
     if t.dtype != F32 or tuple(t.shape) != (n,) or not t.is_contiguous():
@@ -518,12 +535,15 @@ class Fp8Weight:
         return (c.float() * s.float().repeat_interleave(128, 0)[:self.N].repeat_interleave(128, 1)[:, :self.K]).to(dtype)
 
 
-def pack_weight_fp8(w, transposed=False):
-    """w [N, K] f32 / bf16 -> Fp8Weight (once per weight); transposed: keep the codes of w^T too, for gemm_fp8_dgrad"""
+def pack_weight_fp8(w, transposed=False, into=None):
+    """w [N, K] f32 / bf16 -> Fp8Weight (once per weight); transposed: keep the codes of w^T too, for gemm_fp8_dgrad; into: a handle of the same
+    shape, device and `transposed` whose memory is overwritten"""
     ld = _rows(w, "weight")
     if w.shape[0] < 1 or w.shape[1] < 1:
         raise ValueError(f"weight is empty: {tuple(w.shape)}")
-    o = Fp8Weight(w.shape[0], w.shape[1], w.device, transposed)
+    if into is not None and (into.N, into.K, into.codes.device, into.codes_t is not None) != (*w.shape, w.device, bool(transposed)):
+        raise ValueError(f"into holds a weight [{into.N}, {into.K}] on {into.codes.device}, not one like {tuple(w.shape)}")
+    o = copy.copy(into) if into is not None else Fp8Weight(w.shape[0], w.shape[1], w.device, transposed)
     check(lib().fdmi_pack_fp8(ptr(w), int(w.dtype == F32), ld, o.N, o.K, ptr(o.codes), ptr(o.scales), ptr(o.codes_t), ptr(o.scales_t),
                               _stream()))
     return o
@@ -560,6 +580,8 @@ def _fp8_rows_of(d, A, K, what, gated=False):
     M, cols = A.shape
     if cols != K:
         raise ValueError(f"{what} has {cols} columns, the weight contracts over {K}")
+    if M > 1 << 30:
+        raise ValueError(f"{what} has {M} rows: at most 2^30")
     d.M, d.x, d.x_f32 = M, A.data_ptr(), A.dtype == F32
     n = _pad(M, 16) * (_pad(K, 128) // 128)
     if not gated and not lib().fdmi_fp8_scratch_bytes(M, K):
@@ -581,6 +603,10 @@ def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what
         d.ldc = _rows(out, "out")
         if tuple(out.shape) != (M, N):
             raise ValueError(f"out: need [{M}, {N}], got {tuple(out.shape)}")
+        if not isinstance(A, Fp8Rows) and _overlap(A, out):
+            raise ValueError(f"out and {what} share memory")       # (workgroups read A while others already write)
+        if residual is not None and _overlap(residual, out) and (residual.data_ptr(), residual.stride()) != (out.data_ptr(), out.stride()):
+            raise ValueError("out may be the residual, but not share a part of its memory")
     d.N, d.K, d.C, d.out_f32, d.act = N, K, out.data_ptr(), out.dtype == F32, act
     d.W, d.sw = _here(codes, "weight").data_ptr(), scales.data_ptr()
     if bias is not None:
@@ -599,7 +625,8 @@ def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what
 
 def gemm_fp8(A, W, *, bias=None, residual=None, act=ACT_NONE, out=None, out_f32=False):
     """act(A W^T + bias) or A W^T + bias + residual with 8-bit operands: A Fp8Rows, or [M, K] bf16 / f32 rows that the call quantises;
-    W Fp8Weight; bias [N] f32; residual and out [M, N] of one type (bf16, or f32 with out_f32).  fp32 sums, one rounding."""
+    W Fp8Weight; bias [N] f32; residual and out [M, N] of one type (bf16, or f32 with out_f32); out may be the residual, not A.  fp32 sums, one
+    rounding."""
     return _fp8_product(A, W.K, W.N, W.codes, W.scales, bias, residual, act, out, out_f32, "A")
 
 
@@ -672,6 +699,8 @@ def embed_bwd(dy, ids, V, scale=1.0, out=None):
         if tuple(out.shape) != (V, D):
             raise ValueError(f"out: need [{V}, {D}], got {tuple(out.shape)}")
         ldg = _rows(out, "out", (F32,))
+        if _overlap(rows, out):
+            raise ValueError("out and dy share memory")
     else:
         out, ldg = torch.empty((V, D), dtype=F32, device=dy.device), D
     L = lib()

@@ -359,6 +359,39 @@ def test_two_runs_are_bit_identical_and_a_graph_replays_them():
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
 
 
+def test_results_over_operands():
+    """out over A is refused, out over the residual is the same rows or refused, other columns of one buffer are fine"""
+    ops = _ops()
+    W = ops.pack_weight_fp8(_rand(64, 64, seed=1).cuda())
+    for M in (3, 40):
+        x, big = _rand(M, 64, seed=2, dtype=BF16).cuda(), torch.zeros(M, 160, dtype=BF16, device="cuda")
+        with pytest.raises(ValueError, match="share"):
+            ops.gemm_fp8(x, W, out=x)
+        with pytest.raises(ValueError, match="share"):
+            ops.gemm_fp8(big[:, :64], W, out=big[:, 63:127])
+        with pytest.raises(ValueError, match="residual"):
+            ops.gemm_fp8(x, W, residual=big[:, :64], out=big[:, 8:72])
+        want, r = ops.gemm_fp8(x, W), _rand(M, 64, seed=3, dtype=BF16).cuda()
+        big[:, :64], big[:, 128:] = x, 5.0
+        assert torch.equal(ops.gemm_fp8(big[:, :64], W, out=big[:, 64:128]), want)
+        assert torch.equal(big[:, :64], x) and bool((big[:, 128:] == 5.0).all())
+        both = ops.gemm_fp8(x, W, residual=r)
+        assert torch.equal(ops.gemm_fp8(x, W, residual=r, out=r), both) and torch.equal(r, both)
+
+
+def test_rows_beyond_two_to_the_32_bytes():
+    ops = _ops()
+    M, reps, N, K = 1000, 1070, 72, 4096                               # 1070000 rows: 8.8e9 bytes of bf16, 4.4e9 of codes
+    x, w = _rand(M, K, seed=1, dtype=BF16).cuda(), ops.pack_weight_fp8((_rand(N, K, seed=2) * K ** -0.5).cuda())
+    X = x.repeat(reps, 1)
+    y = ops.gemm_fp8(X, w)
+    assert torch.equal(y.view(reps, M, N), y[:M].expand(reps, M, N))    # the same rows, whatever their place
+    xv, wv = ops.quant_fp8(x).values(F32).double(), w.values(F32).double()
+    _check(y[-M:], _np(xv) @ _np(wv).T, _np(xv), _np(wv), BF16)
+    h = ops.gated_fp8(X, w, w).values().view(reps, M, N)
+    assert torch.equal(h, h[:1].expand(reps, M, N)) and torch.equal(h[0], ops.gated_fp8(X[:64000], w, w).values()[:M])
+
+
 def test_refusals_on_the_gpu():
     ops = _ops()
     W = ops.pack_weight_fp8(_rand(64, 130).cuda())

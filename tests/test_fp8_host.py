@@ -36,6 +36,23 @@ def test_gemm_fp8_refuses(kw):
     assert b"gemm_fp8" in L.fdmi_last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(M=(1 << 30) + 1), dict(N=(1 << 17) + 1, ldc=1 << 18), {**GATED, "N": (1 << 17) + 1}])
+def test_gemm_fp8_refuses_sizes_beyond_its_indexes(kw):
+    L = _lib().lib()
+    assert L.fdmi_gemm_fp8(C.byref(_desc(**kw)), None) != 0 and b"gemm_fp8" in L.fdmi_last_error()
+    assert L.fdmi_quant_fp8(P, 0, 130, None, 0.0, P, P, (1 << 30) + 1, 130, None) != 0 and b"quant_fp8" in L.fdmi_last_error()
+
+
+def test_shared_memory_of_rows_is_seen():
+    """(what a product refuses of out: the check itself, on host tensors)"""
+    from flash_diffusion_amd.ops import _overlap
+    b = torch.zeros(10, 40)
+    assert _overlap(b, b) and _overlap(b[:, :20], b[:, 19:]) and _overlap(b[2:5], b[4:8]) and _overlap(b[:, 5:9], b[3:4, 8:30])
+    assert not _overlap(b[:, :20], b[:, 20:]) and not _overlap(b[:, 20:], b[:, :20]) and not _overlap(b[:5], b[5:]) and not _overlap(b, torch.zeros(10, 40))
+    assert not _overlap(b[2:, 3:7], b[:-2, 7:20]) and not _overlap(b[:0], b) and _overlap(b[1:9:2, :20], b[1:9, :10])
+    assert _overlap(b[:9, 30:40], b.view(-1)[35:35 + 9 * 40].view(9, 40)[:, :10])          # runs over the end of a row
+
+
 def test_empty_calls_are_accepted_without_a_gpu():
     L = _lib().lib()
     assert L.fdmi_gemm_fp8(C.byref(_desc(M=0)), None) == 0

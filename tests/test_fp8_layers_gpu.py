@@ -145,6 +145,70 @@ def test_packing_under_capture_is_refused():
         w + 1
 
 
+def test_a_captured_graph_sees_a_weight_that_is_packed_again():
+    from flash_diffusion_amd import ops
+    from flash_diffusion_amd.fp8 import PackedFp8
+    w, x, p = _rand(70, 260).cuda(), _rand(40, 260, seed=1).cuda(), PackedFp8()
+    p(w)
+    ops.gemm_fp8(x, p(w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.gemm_fp8(x, p(w))
+    for seed in (2, 3):
+        w.copy_(_rand(70, 260, seed=seed))
+        want = ops.gemm_fp8(x, p(w))                         # packs again
+        noise = [torch.full((70000,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]   # (memory that had been freed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and len(noise) == 8
+    q = p(w)
+    w = _rand(71, 260).cuda()                                # another shape: its own memory
+    assert p(w).N == 71 and q.N == 70
+    with pytest.raises(ValueError, match="into"):
+        ops.pack_weight_fp8(w, into=q)
+    with pytest.raises(ValueError, match="into"):
+        ops.pack_weight_fp8(w, True, into=p(w))
+
+
+def test_layers_under_a_captured_backward():
+    """forward and backward of lookup and 8-bit layer in one graph, replayed with new inputs between eager work"""
+    from flash_diffusion_amd.fp8 import Fp8Linear, TokenEmbedding, _LookupFn
+    emb, lin = TokenEmbedding(50, 136).cuda(), Fp8Linear(_rand(40, 136, seed=1).cuda(), _rand(40, seed=2).cuda())
+    ids, dy = torch.randint(0, 50, (3, 30)).cuda(), _rand(3, 30, 40, seed=3, dtype=BF16).cuda()
+
+    def step():
+        w = emb.weight.detach().requires_grad_()             # (a leaf of this graph alone)
+        out = lin(_LookupFn.apply(w, None, ids, 0.5, BF16))
+        return out.detach(), torch.autograd.grad(out, w, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (4, 5, 6):
+        ids.copy_(torch.randint(0, 50, (3, 30), generator=torch.Generator().manual_seed(seed)))
+        dy.copy_(_rand(3, 30, 40, seed=seed))
+        emb.weight.data.copy_(_rand(50, 136, seed=seed))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_second_derivatives_are_refused():
+    from flash_diffusion_amd.fp8 import Fp8Linear, TokenEmbedding
+    lin, emb = Fp8Linear(_rand(40, 136, seed=1).cuda()), TokenEmbedding(9, 8).cuda()
+    x = _rand(5, 136).cuda().requires_grad_()
+    for leaf, y in ((x, lin(x)), (emb.weight, emb(torch.tensor([1, 2], device="cuda"), dtype=F32))):
+        (g,) = torch.autograd.grad((y * y).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
 # ---- the trained table in front of frozen 8-bit layers ---------------------------------------------------------------------------------
 def test_a_token_table_learns_through_frozen_8_bit_layers():
     """lookup -> two linear maps -> a weighted sum: the table's gradient against the formula in 64 bits on the values that the layers hold"""
