@@ -674,7 +674,7 @@ __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
   constexpr int DEPTH = MT * 2 + NT * 2 <= 4 ? 4 : MT * 2 + NT * 2 <= 8 ? 2 : 1, LD = NT * 16 + 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t panel = (int64_t)a.Kb * 2048;
-  const int Mt = (a.M + 15) >> 4, mt0 = blockIdx.y * MT, nt0 = blockIdx.x * NT;
+  const int Mt = (a.M + 15) >> 4, across = (a.N + NT * 16 - 1) / (NT * 16), mt0 = blockIdx.x / across * MT, nt0 = blockIdx.x % across * NT;
   const int64_t Mp = (int64_t)Mt * 16, Ng = (int64_t)((a.N + 255) >> 8) * 8;
   constexpr bool FUSED = !std::is_void<RAW>::value;
   static_assert(!FUSED || MT == 1, "sixteen rows");
@@ -789,8 +789,9 @@ int launch_stream(const Fp8GemmArgs& a, hipStream_t st) {
   static std::atomic<uint64_t> allowed;
   if (const int rc = allow_lds((const void*)fp8_stream_kernel<MT, NT, WIDE, RAW>, most, allowed)) return rc;
   const int codes = std::is_void<RAW>::value ? 0 : a.M * a.Kb * 129, smem = join > codes ? join : codes;
-  const dim3 grid(cdiv(a.N, NT * 16), cdiv(a.M, MT * 16));
-  hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE, RAW>), grid, dim3(512), smem, st, a);
+  const int64_t grid = (int64_t)cdiv(a.N, NT * 16) * cdiv(a.M, MT * 16);   // (in one dimension: the second holds 65535)
+  FDMI_CHECK(grid < (1ll << 31), "gemm_fp8: too many tiles");
+  hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE, RAW>), dim3((unsigned)grid), dim3(512), smem, st, a);
   FDMI_HIP(hipGetLastError());
   return 0;
 }

@@ -392,6 +392,19 @@ def test_rows_beyond_two_to_the_32_bytes():
     assert torch.equal(h, h[:1].expand(reps, M, N)) and torch.equal(h[0], ops.gated_fp8(X[:64000], w, w).values()[:M])
 
 
+@pytest.mark.parametrize("N,K", [(8, 64), (40, 100)])
+def test_many_short_rows(N, K):
+    """more row tiles than the second dimension of a grid holds"""
+    ops = _ops()
+    M, reps = 2 ** 10 + 16, 2100
+    x, w = _rand(M, K, seed=1, dtype=BF16).cuda(), ops.pack_weight_fp8((_rand(N, K, seed=2) * K ** -0.5).cuda())
+    for f32 in (False, True):
+        y = ops.gemm_fp8(x.repeat(reps, 1), w, out_f32=f32).view(reps, M, N)
+        xv, wv = _np(ops.quant_fp8(x).values(F32)), _np(w.values(F32))
+        _check(y[-1], xv @ wv.T, xv, wv, F32 if f32 else BF16)
+        assert torch.equal(y, y[:1].expand(reps, M, N))
+
+
 def test_refusals_on_the_gpu():
     ops = _ops()
     W = ops.pack_weight_fp8(_rand(64, 130).cuda())
