@@ -496,9 +496,7 @@ int fdmi_gemm_fp8(const fdmi_fp8_desc* d, void* stream) {
     a.bias = d->bias; a.residual = d->residual; a.ldr = d->ldr; a.C = d->C; a.ldc = d->ldc; a.out_f32 = d->out_f32; a.act = d->act;
   }
   if (fused) {
-    const int es = d->x_f32 ? 4 : 2;
     a.x = d->x; a.ldxr = d->ldxr; a.x_f32 = d->x_f32; a.K = d->K;
-    a.xvec = ((uintptr_t)d->x & 15) == 0 && d->ldxr * es % 16 == 0;
   } else if (d->x) {
     const int rc = launch_quant_fp8(d->x, d->x_f32, d->ldxr, nullptr, 0.f, (uint8_t*)d->X, (uint8_t*)d->sx, d->M, d->K, (hipStream_t)stream);
     if (rc) return rc;

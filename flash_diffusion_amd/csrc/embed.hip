@@ -19,6 +19,11 @@ constexpr int32_t NONE = 0x7fffffff;   // key of an id outside the table: behind
 __device__ __forceinline__ int64_t id_at(const void* ids, int ids64, int64_t i) {
   return ids64 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
 }
+// VEC columns with 16-byte accesses at any address that an element may have.  A lane whose columns would pass the end
+// of a row of D >= VEC takes the row's last VEC columns instead, and shares some of them with its neighbour
+typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T, int VEC>
 __device__ __forceinline__ void load_cols(const T* p, float v[VEC]) {
   if constexpr (VEC == 1) {
@@ -27,15 +32,12 @@ __device__ __forceinline__ void load_cols(const T* p, float v[VEC]) {
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int k = 0; k < VEC; k += 4) {
-      const float4 t = *(const float4*)(p + k);
-      v[k] = t.x; v[k + 1] = t.y; v[k + 2] = t.z; v[k + 3] = t.w;
-    }
-  } else if constexpr (VEC == 4) {
-    const u16x4 t = *(const u16x4*)p;
+      const f32x4_any t = *(const f32x4_any*)(p + k);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = bf2f(t[k]);
+      for (int e = 0; e < 4; ++e) v[k + e] = t[e];
+    }
   } else {
-    const u16x8 t = *(const u16x8*)p;
+    const u16x8_any t = *(const u16x8_any*)p;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = bf2f(t[k]);
   }
@@ -52,7 +54,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t 
   const T* row = table + (ok ? id : 0) * ldt;
   const float* pr = pos ? pos + (i % pos_rows) * ldp : nullptr;
   O* o = out + i * D;
-  for (int c = (threadIdx.x & 63) * VEC; c < D; c += 64 * VEC) {
+  for (int c0 = (threadIdx.x & 63) * VEC; c0 < D; c0 += 64 * VEC) {
+    const int c = c0 + VEC <= D ? c0 : D - VEC;
     float v[VEC], q[VEC];
     load_cols<T, VEC>(row + c, v);
 #pragma unroll
@@ -64,10 +67,10 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t 
       if constexpr (sizeof(O) == 2) o[c] = f2bf(v[0]);
       else o[c] = v[0];
     } else if constexpr (sizeof(O) == 2) {
-      *(uint4*)(o + c) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+      *(u32x4_any*)(o + c) = (u32x4_any){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
     } else {
-      *(float4*)(o + c) = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4*)(o + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      *(f32x4_any*)(o + c) = (f32x4_any){v[0], v[1], v[2], v[3]};
+      *(f32x4_any*)(o + c + 4) = (f32x4_any){v[4], v[5], v[6], v[7]};
     }
   }
 }
@@ -175,19 +178,32 @@ __global__ __launch_bounds__(PARTS ? 1024 : 256) void order_kernel(const void* i
   }
 }
 
+// a lane's VEC columns of a row of D, from `col` on as load_cols takes them (v: of the row's last VEC, if fewer are left)
 template <int VEC>
-__device__ __forceinline__ void put_row(float* o, const float v[VEC], float scale, int accumulate) {
-  if constexpr (VEC == 1) {
+__device__ __forceinline__ void put_row(float* row, int col, int D, const float v[VEC], float scale, int accumulate) {
+  float* o = row + col;
+  if (VEC == 1) {
     *o = accumulate ? fmaf(scale, v[0], *o) : scale * v[0];
-  } else {
+  } else if (col + VEC <= D) {
 #pragma unroll
     for (int k = 0; k < VEC; k += 4) {
-      float4 t = make_float4(scale * v[k], scale * v[k + 1], scale * v[k + 2], scale * v[k + 3]);
+      f32x4_any t = {scale * v[k], scale * v[k + 1], scale * v[k + 2], scale * v[k + 3]};
       if (accumulate) {
-        const float4 b = *(const float4*)(o + k);
-        t = make_float4(fmaf(scale, v[k], b.x), fmaf(scale, v[k + 1], b.y), fmaf(scale, v[k + 2], b.z), fmaf(scale, v[k + 3], b.w));
+        const f32x4_any b = *(const f32x4_any*)(o + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = fmaf(scale, v[k + e], b[e]);
       }
-      *(float4*)(o + k) = t;
+      *(f32x4_any*)(o + k) = t;
+    }
+  } else {                                       // its own columns only (added to once), from the last on
+    float w[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[k] = v[k];
+#pragma unroll 1
+    for (int c = D - 1; c >= col; --c) {
+      row[c] = accumulate ? fmaf(scale, w[VEC - 1], row[c]) : scale * w[VEC - 1];
+#pragma unroll
+      for (int k = VEC - 1; k > 0; --k) w[k] = w[k - 1];
     }
   }
 }
@@ -216,20 +232,20 @@ __device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const int32_t* 
     float* row = g + (v0 + __ffs(todo) - 1) * ldg;
     for (int c = threadIdx.x * VEC; c < D; c += 256 * VEC) {
       if constexpr (VEC == 1) row[c] = 0.f;
-      else *(float4*)(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+      else *(f32x4_any*)(row + (c + VEC <= D ? c : D - VEC)) = (f32x4_any){0.f, 0.f, 0.f, 0.f};
     }
   }
 }
 
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy, const int32_t* sid, const int32_t* spos, int64_t n, int D,
+__global__ __launch_bounds__(256, VEC == 8 ? 4 : 5) void run_sum_kernel(const T* dy, int64_t lddy, const int32_t* sid, const int32_t* spos, int64_t n, int D,
                                                       int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part, int summers,
                                                       int64_t V) {
   if ((int)blockIdx.x >= summers) return zero_rows<(VEC > 1 ? 4 : 1)>(((int64_t)blockIdx.x - summers) * ZROWS, V, sid, n, D, g, ldg);
   __shared__ float head[4][64 * VEC];            // per wave: its share of the run that came in over its left edge
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t c = blockIdx.x / col_groups, p0 = c * CHUNK + wave * ROWS;
-  const int col = ((int)(blockIdx.x - c * col_groups) * 64 + lane) * VEC, mine = col < D ? col : 0;
+  const int col = ((int)(blockIdx.x - c * col_groups) * 64 + lane) * VEC, mine = col + VEC <= D ? col : D - VEC;
   const int count = (int)(p0 + ROWS < n ? ROWS : p0 < n ? n - p0 : 0);
   int32_t edge[5];                               // the key at each wave's left edge, and behind the chunk
 #pragma unroll
@@ -262,7 +278,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy,
 #pragma unroll
           for (int k = 0; k < VEC; ++k) out[k] = sum[k];
         } else if (col < D) {
-          put_row<VEC>(g + (int64_t)id[q] * ldg + col, sum, scale, accumulate);
+          put_row<VEC>(g + (int64_t)id[q] * ldg, col, D, sum, scale, accumulate);
         }
       }
 #pragma unroll
@@ -280,15 +296,15 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* dy, int64_t lddy,
   if (leaves != NONE) {
     add_heads(wave + 1, leaves, out);
     if (col < D) {
-      if (edge[4] == leaves) put_row<VEC>(part + (c * 2 + 1) * D + col, out, 1.f, 0);
-      else put_row<VEC>(g + (int64_t)leaves * ldg + col, out, scale, accumulate);
+      if (edge[4] == leaves) put_row<VEC>(part + (c * 2 + 1) * D, col, D, out, 1.f, 0);
+      else put_row<VEC>(g + (int64_t)leaves * ldg, col, D, out, scale, accumulate);
     }
   }
   if (wave == 0 && before == edge[0] && before != NONE) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) out[k] = head[0][k * 64 + lane];
     add_heads(1, before, out);
-    if (col < D) put_row<VEC>(part + (c * 2) * D + col, out, 1.f, 0);
+    if (col < D) put_row<VEC>(part + (c * 2) * D, col, D, out, 1.f, 0);
   }
 }
 
@@ -301,7 +317,7 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
                                                                    int64_t ldg, const float* part) {
   __shared__ float share[JOINERS][64 * VEC];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = (blockIdx.y * 64 + lane) * VEC;
+  const int col = (blockIdx.y * 64 + lane) * VEC, at = col + VEC <= D ? col : D - VEC;
   const int64_t chunks = (n + CHUNK - 1) / CHUNK, k0 = (int64_t)blockIdx.x * JOINERS, c = k0 + (lane & (JOINERS - 1));
   auto key = [&](int64_t p) { return sid[p < n ? p : n - 1]; };         // (all asked for at once)
   const int32_t before = c > 0 ? key(c * CHUNK - 1) : -1, last = key((c + 1) * CHUNK - 1), next = key((c + 1) * CHUNK);
@@ -315,7 +331,7 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
     for (int64_t k = from; k < to; k += DEEP) {
       float v[DEEP][VEC];
 #pragma unroll
-      for (int q = 0; q < DEEP; ++q) load_cols<float, VEC>(part + ((k + q < to ? k + q : to - 1) * 2) * D + col, v[q]);
+      for (int q = 0; q < DEEP; ++q) load_cols<float, VEC>(part + ((k + q < to ? k + q : to - 1) * 2) * D + at, v[q]);
 #pragma unroll
       for (int q = 0; q < DEEP; ++q)
 #pragma unroll
@@ -346,9 +362,9 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
     const int64_t end = end_of(k + 1, id, 1);
     if (col < D) {
       float s[VEC];
-      load_cols<float, VEC>(part + (k * 2 + 1) * D + col, s);
+      load_cols<float, VEC>(part + (k * 2 + 1) * D + at, s);
       add_rows(k + 1, end, s);
-      put_row<VEC>(g + (int64_t)id * ldg + col, s, scale, accumulate);
+      put_row<VEC>(g + (int64_t)id * ldg, col, D, s, scale, accumulate);
     }
   }
   while (longs) {
@@ -362,7 +378,7 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s[e] = 0.f;
     if (col < D) {
-      if (wave == 0) load_cols<float, VEC>(part + (k * 2 + 1) * D + col, s);
+      if (wave == 0) load_cols<float, VEC>(part + (k * 2 + 1) * D + at, s);
       add_rows(from, to, s);
     }
 #pragma unroll
@@ -372,13 +388,11 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
       for (int q = 1; q < JOINERS; ++q)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s[e] += share[q][lane * VEC + e];
-      put_row<VEC>(g + (int64_t)id * ldg + col, s, scale, accumulate);
+      put_row<VEC>(g + (int64_t)id * ldg, col, D, s, scale, accumulate);
     }
     __syncthreads();
   }
 }
-
-bool aligned16(const void* p, int64_t ld_bytes) { return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0; }
 
 }  // namespace
 
@@ -387,7 +401,7 @@ int launch_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t
   if (n == 0) return 0;
   const int64_t blocks = (n + 3) / 4;
   FDMI_CHECK(blocks < (1ll << 31), "embed_fwd: too many tokens");
-  const bool vec = D % 8 == 0 && aligned16(table, ldt * (table_f32 ? 4 : 2)) && (!pos || aligned16(pos, ldp * 4)) && aligned16(out, 0);
+  const bool vec = D >= 8;
 #define EMB_FWD(T, O, VEC) hipLaunchKernelGGL((embed_fwd_kernel<T, O, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)table, V, D, ldt, \
                                               ids, ids64, n, scale, pos, pos_rows, ldp, (O*)out)
   if (table_f32) { if (out_f32) { if (vec) EMB_FWD(float, float, 8); else EMB_FWD(float, float, 1); }
@@ -420,8 +434,7 @@ static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* id
   } else if (n > 0) {
     hipLaunchKernelGGL(order_kernel<false>, dim3(cdiv(n, 64)), dim3(256), 0, st, ids, ids64, n, V, nullptr, nullptr, sid, spos);
   }
-  const bool vec = D % 4 == 0 && aligned16(dy, lddy * 4) && (dy_f32 || lddy % 4 == 0) && aligned16(grad, ldg * 4);
-  const bool vec8 = vec && !dy_f32 && D % 8 == 0 && lddy % 8 == 0;                       // (16 bytes of a bf16 row per lane)
+  const bool vec = D >= 8, vec8 = vec && !dy_f32;                                        // (16 bytes of a row per lane)
   const int groups = cdiv(D, vec8 ? 512 : vec ? 256 : 64);
   const int64_t chunks = (n + CHUNK - 1) / CHUNK, summers = chunks * groups, blocks = summers + (accumulate ? 0 : (V + ZROWS - 1) / ZROWS);
   FDMI_CHECK(blocks < (1ll << 31), "embed_bwd: too many tokens");
@@ -430,7 +443,7 @@ static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* id
 #define EMB_SUM(T, VEC) hipLaunchKernelGGL((run_sum_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)dy, lddy, sid, spos, n, D, \
                                            groups, scale, accumulate, grad, ldg, part, (int)summers, V)
   if (vec) {
-    if (dy_f32) EMB_SUM(float, 4); else if (vec8) EMB_SUM(bf16_t, 8); else EMB_SUM(bf16_t, 4);
+    if (dy_f32) EMB_SUM(float, 4); else EMB_SUM(bf16_t, 8);
     if (chunks > 1) hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
   } else {
     if (dy_f32) EMB_SUM(float, 1); else EMB_SUM(bf16_t, 1);

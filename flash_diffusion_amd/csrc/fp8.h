@@ -9,7 +9,7 @@ struct Fp8GemmArgs {
   const uint8_t* W = nullptr; const uint8_t* sw = nullptr;
   const uint8_t* W2 = nullptr; const uint8_t* sw2 = nullptr;
   int M = 0, N = 0, Kb = 0;
-  const void* x = nullptr; int64_t ldxr = 0; int x_f32 = 0, K = 0; bool xvec = false;   // unquantised rows in X's place (fp8_fused problems)
+  const void* x = nullptr; int64_t ldxr = 0; int x_f32 = 0, K = 0;   // unquantised rows in X's place (fp8_fused problems)
   const float* bias = nullptr;
   const void* residual = nullptr; int64_t ldr = 0;             // of C's type
   void* C = nullptr; int64_t ldc = 0; int out_f32 = 0;

@@ -47,17 +47,26 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
   return (uint32_t)r;
 }
 
-// eight consecutive elements of a row from column k on; columns >= K read as zero.  vec: rows start 16-byte aligned
+// 16-byte accesses at any address that an element may have
+typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// eight consecutive elements of a row from column k on; columns >= K read as zero
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int k, int K, bool vec, float v[8]) {
-  if (vec && k + 8 <= K) {
+__device__ __forceinline__ void load8(const T* p, int k, int K, float v[8]) {
+  if (k + 8 <= K) {
     if constexpr (sizeof(T) == 2) {
-      const u16x8 t = *(const u16x8*)(p + k);
+      const u16x8_any t = *(const u16x8_any*)(p + k);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = bf2f(t[i]);
     } else {
-      const float4 a = *(const float4*)(p + k), b = *(const float4*)(p + k + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      const f32x4_any a = *(const f32x4_any*)(p + k), b = *(const f32x4_any*)(p + k + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
     }
   } else {
 #pragma unroll
@@ -70,9 +79,9 @@ __device__ __forceinline__ void load8(const T* p, int k, int K, bool vec, float 
 
 // sixteen consecutive elements of a row from column k on, as load8
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, int k, int K, bool vec, float v[16]) {
-  load8(p, k, K, vec, v);
-  load8(p, k + 8, K, vec, v + 8);
+__device__ __forceinline__ void load16(const T* p, int k, int K, float v[16]) {
+  load8(p, k, K, v);
+  load8(p, k + 8, K, v + 8);
 }
 // a block of 128 held by eight lanes, 16 values each, that differ in the lane bits o0, o1, o2: its scale byte.  Infinities are rare: they are
 // seen in the maximum (fmax drops a NaN), only then replaced by NaN and the maximum taken again over the finite values; the values
@@ -112,7 +121,7 @@ __device__ __forceinline__ uint4 codes16(const float v[16], float up) {
 // 64 consecutive bytes).  NORM: y = x * rsqrt(mean(x^2) + eps) * w in fp32 first, each wave summing one row's squares.
 template <typename T, bool NORM>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, int64_t ldx, const float* w, float eps, uint8_t* q, uint8_t* s, int64_t M,
-                                                         int64_t Mp, int K, int Kb, bool vec, bool wvec) {
+                                                         int64_t Mp, int K, int Kb) {
   __shared__ float rs[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t m0 = (int64_t)blockIdx.x * 4;
@@ -121,7 +130,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, int64_t ldx
     float ss = 0.f, v[8];
 #pragma unroll 4
     for (int k = lane * 8; k < K; k += 512) {
-      load8(row, k, K, vec, v);
+      load8(row, k, K, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
     }
@@ -138,10 +147,10 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, int64_t ldx
   for (int k0 = first; k0 < stop; k0 += 2048) {
     float v[2][16], g[2][16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) load16(row, k0 + h * 1024 + c * 16, cols, vec, v[h]);
+    for (int h = 0; h < 2; ++h) load16(row, k0 + h * 1024 + c * 16, cols, v[h]);
     if constexpr (NORM) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) load16(w, k0 + h * 1024 + c * 16, K, wvec, g[h]);
+      for (int h = 0; h < 2; ++h) load16(w, k0 + h * 1024 + c * 16, K, g[h]);
       const float rr = rs[r];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -254,10 +263,8 @@ __device__ __forceinline__ float act_of(int act, float v) {
   }
 }
 
-// eight consecutive columns of one row, with 16-byte accesses at any address that an element may have (rows of odd lengths included: turned
-// round in LDS and stored by single columns, 4096 x 4100 x 4096 took 147 us): the residual (16 bytes of bf16, 32 of fp32) ...
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+// eight consecutive columns of one row, rows of odd lengths included (turned round in LDS and stored by single columns, 4096 x 4100 x 4096 took
+// 147 us instead of 79): the residual (16 bytes of bf16, 32 of fp32) ...
 template <bool F32>
 __device__ __forceinline__ void load_res8(const Fp8GemmArgs& a, int m, int n, uint4 r[F32 ? 2 : 1]) {
   const char* p = (const char*)a.residual + ((int64_t)m * a.ldr + n) * (F32 ? 4 : 2);
@@ -715,7 +722,7 @@ __global__ __launch_bounds__(512) void fp8_stream_kernel(const Fp8GemmArgs a) {
     for (int u = threadIdx.x; u < a.M * per; u += 512) {
       const int m = u / per, c = u - m * per;
       float v[16];
-      load16((const RAW*)a.x + (int64_t)m * a.ldxr, c * 16, a.K, a.xvec, v);
+      load16((const RAW*)a.x + (int64_t)m * a.ldxr, c * 16, a.K, v);
       const int byte = block_scale(v, 1, 2, 4);
       *(uint4*)(smem + (c * a.M + m) * 16) = codes16(v, scale_up(byte));
       if ((c & 7) == 0) sq[(c >> 3) * a.M + m] = (uint8_t)byte;
@@ -796,19 +803,16 @@ int launch_stream(const Fp8GemmArgs& a, hipStream_t st) {
   return 0;
 }
 
-bool aligned(const void* p, int64_t ld_bytes, int to) { return ((uintptr_t)p % to) == 0 && (ld_bytes % to) == 0; }
-
 }  // namespace
 
 int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, float eps, uint8_t* q, uint8_t* s, int64_t M, int K,
                      hipStream_t st) {
   if (M == 0) return 0;
-  const bool vec = aligned(x, ldx * (x_f32 ? 4 : 2), 16), wvec = ((uintptr_t)norm % 16) == 0;
   const int Kb = cdiv(K, 128);
   const int64_t Mp = (M + 15) / 16 * 16, rows4 = (M + 3) / 4;
   FDMI_CHECK(rows4 < (1ll << 31) && cdiv(Kb, 16) < 65536, "quant_fp8: too many rows or columns");
   const dim3 grid((unsigned)rows4, norm ? 1 : cdiv(Kb, 16));
-#define FP8_QUANT(T, NORM) hipLaunchKernelGGL((quant_rows_kernel<T, NORM>), grid, dim3(256), 0, st, (const T*)x, ldx, norm, eps, q, s, M, Mp, K, Kb, vec, wvec)
+#define FP8_QUANT(T, NORM) hipLaunchKernelGGL((quant_rows_kernel<T, NORM>), grid, dim3(256), 0, st, (const T*)x, ldx, norm, eps, q, s, M, Mp, K, Kb)
   if (norm) { if (x_f32) FP8_QUANT(float, true); else FP8_QUANT(bf16_t, true); }
   else { if (x_f32) FP8_QUANT(float, false); else FP8_QUANT(bf16_t, false); }
 #undef FP8_QUANT
