@@ -20,7 +20,6 @@ import torch.nn as nn
 
 from . import ops
 from .conditioners import BaseConditioner
-from .fp8 import TokenEmbedding
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -69,7 +68,7 @@ class _Layer(nn.Module):
 class _Embeddings(nn.Module):
     def __init__(self, vocab, d, maxpos):
         super().__init__()
-        self.token_embedding = TokenEmbedding(vocab, d)
+        self.token_embedding = nn.Embedding(vocab, d)
         self.position_embedding = nn.Embedding(maxpos, d)
         self.register_buffer("position_ids", torch.arange(maxpos).unsqueeze(0), persistent=False)
 
@@ -123,11 +122,11 @@ class MiCLIPTextModel(nn.Module):
         pos = emb.position_embedding.weight[:S].float()
         hidden: List[torch.Tensor] = []
         if output_hidden_states:               # hidden_states[0] is the embedding in fp32
-            h32 = emb.token_embedding(input_ids, pos=pos, dtype=F32)
+            h32 = ops.embed_fwd(emb.token_embedding.weight, input_ids, pos=pos, dtype=F32, wrap=True)
             hidden.append(h32)
             h = self._act(h32.view(B * S, D))
         else:
-            h = emb.token_embedding(input_ids, pos=pos, dtype=dt).view(B * S, D)
+            h = ops.embed_fwd(emb.token_embedding.weight, input_ids, pos=pos, dtype=dt, wrap=True).view(B * S, D)
         eps = c.layer_norm_eps
         for lyr in tm.encoder.layers:
             a = lyr.self_attn

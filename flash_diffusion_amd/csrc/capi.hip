@@ -520,6 +520,6 @@ int fdmi_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, in
   FDMI_CHECK(V >= 1 && V < 0x7fffffff && D >= 1 && n >= 0 && n < (1ll << 31), "embed_bwd: need a gradient [V][D] and 0 <= n < 2^31 ids");
   FDMI_CHECK(grad && ldg >= D, "embed_bwd: gradient rows shorter than D");
   FDMI_CHECK(n == 0 || (dy && lddy >= D && ids && ws && ((uintptr_t)ws & 15) == 0), "embed_bwd: null operand, short rows or unaligned scratch");
-  return launch_embed_bwd(dy, dy_f32, lddy, ids, ids64, n, V, D, scale, accumulate, grad, ldg, ws, (hipStream_t)stream);
+  return launch_embed_bwd(dy, dy_f32, lddy, ids, ids64 & 1, n, V, D, scale, accumulate, grad, ldg, ws, (hipStream_t)stream);
 }
 }  // extern "C"

@@ -17,7 +17,7 @@ constexpr int ROWS = 16, CHUNK = 64;   // sorted positions summed by one wave (i
 constexpr int32_t NONE = 0x7fffffff;   // key of an id outside the table: behind all others
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int ids64, int64_t i) {
-  return ids64 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
+  return ids64 & 1 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
 }
 // VEC columns with 16-byte accesses at any address that an element may have.  A lane whose columns would pass the end
 // of a row of D >= VEC takes the row's last VEC columns instead, and shares some of them with its neighbour
@@ -49,7 +49,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t 
                                                         float scale, const float* pos, int64_t pos_rows, int64_t ldp, O* out) {
   const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= n) return;
-  const int64_t id = id_at(ids, ids64, i);
+  int64_t id = id_at(ids, ids64, i);
+  if (ids64 & 2) id += id < 0 ? V : 0;           // counted from the end, as in indexing
   const bool ok = id >= 0 && id < V;
   const T* row = table + (ok ? id : 0) * ldt;
   const float* pr = pos ? pos + (i % pos_rows) * ldp : nullptr;

@@ -662,9 +662,10 @@ def _ids(ids):
     return ids if ids.is_contiguous() else ids.contiguous()
 
 
-def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16):
+def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16, wrap=False):
     """scale * table[ids] (+ pos[t], t the last index of ids) -> [*ids.shape, D] in `dtype`: table [V, D] f32 / bf16, ids int32 / int64,
-    pos [>= ids.shape[-1], D] f32.  An id outside the table gives a row of NaN."""
+    pos [>= ids.shape[-1], D] f32.  An id outside the table gives a row of NaN; wrap: ids -V .. -1 count from
+    its end, as in table[ids]."""
     ld = _rows(table, "table")
     ids = _ids(ids)
     V, D = table.shape
@@ -679,7 +680,7 @@ def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16):
     out = torch.empty((*shape, D), dtype=dtype, device=table.device)
     n = ids.numel()
     if n:
-        check(lib().fdmi_embed_fwd(table.data_ptr(), table.dtype == F32, V, D, ld, ids.data_ptr(), ids.dtype == torch.int64, n, scale, p, S,
+        check(lib().fdmi_embed_fwd(table.data_ptr(), table.dtype == F32, V, D, ld, ids.data_ptr(), (ids.dtype == torch.int64) + 2 * bool(wrap), n, scale, p, S,
                                    ldp, out.data_ptr(), dtype == F32, _stream()))
     return out
 

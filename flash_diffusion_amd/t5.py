@@ -30,7 +30,7 @@ import torch.nn as nn
 
 from . import ops
 from .conditioners import BaseConditioner
-from .fp8 import PackedFp8, TokenEmbedding
+from .fp8 import PackedFp8
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -97,7 +97,7 @@ class _Block(nn.Module):
 class _Stack(nn.Module):
     def __init__(self, vocab, d, inner, heads, ff, gated, n, buckets):
         super().__init__()
-        self.embed_tokens = TokenEmbedding(vocab, d)
+        self.embed_tokens = nn.Embedding(vocab, d)
         self.block = nn.ModuleList([_Block(d, inner, heads, ff, gated, buckets if i == 0 else 0) for i in range(n)])
         self.final_layer_norm = _Norm(d)
 
@@ -127,7 +127,7 @@ class MiT5EncoderModel(nn.Module):
                                       num_heads=num_heads, relative_attention_num_buckets=relative_attention_num_buckets,
                                       relative_attention_max_distance=relative_attention_max_distance,
                                       layer_norm_epsilon=layer_norm_epsilon, feed_forward_proj=feed_forward_proj)
-        self.shared = TokenEmbedding(vocab_size, d_model)
+        self.shared = nn.Embedding(vocab_size, d_model)
         self.encoder = _Stack(vocab_size, d_model, inner, num_heads, d_ff, feed_forward_proj == "gated-gelu", num_layers,
                               relative_attention_num_buckets)
         self.encoder.embed_tokens.weight = self.shared.weight          # tied, as in transformers
@@ -195,7 +195,7 @@ class MiT5EncoderModel(nn.Module):
         assert input_ids.is_cuda, "MiT5EncoderModel runs on the GPU only (no CPU fallback)"
         B, S = input_ids.shape
         D, dt, eps = c.d_model, self.dt, c.layer_norm_epsilon
-        h = self.shared(input_ids, dtype=dt).view(B * S, D)
+        h = ops.embed_fwd(self.shared.weight, input_ids, dtype=dt, wrap=True).view(B * S, D)
         hidden: List[torch.Tensor] = []
         bias = self._position_bias(S, input_ids.device)
         kbias = None

@@ -246,6 +246,7 @@ int64_t fdmi_fp8_scratch_bytes(int64_t M, int K);   /* of codes and scales toget
 /* ---------------- token-embedding lookup and its gradient (csrc/embed.hip) ----------------
  * out[i][:] = scale * table[ids[i]][:] + pos[i mod pos_rows][:]  (table fp32 or bf16 [V][D], pos fp32 or NULL, ids int32 or int64,
  * out bf16 or fp32 [n][D]): the text encoders' token (+ position) embedding.  An id outside [0, V) gives a row of NaN.
+ * ids64: bit 0: the ids are int64; bit 1 (lookup only): ids -V .. -1 count from the end of the table, as in indexing.
  * grad[v][:] (+)= scale * sum over ids[i] == v of dy[i][:], fp32 sums in a fixed order (positions ascending in fixed chunks): two
  * runs are bit-identical.  accumulate = 0 writes every row of grad [V][ldg], 1 adds to the rows that occur.  ws: scratch of
  * fdmi_embed_bwd_ws_bytes(n, D) bytes, 16-byte aligned.                                                                              */

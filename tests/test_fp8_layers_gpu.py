@@ -304,3 +304,21 @@ def test_the_encoders_lookup_is_the_gather_it_replaces():
     ids = torch.randint(0, 300, (3, 50), generator=torch.Generator().manual_seed(3)).cuda()
     assert torch.equal(ops.embed_fwd(w, ids, dtype=F32), w[ids]) and torch.equal(ops.embed_fwd(w, ids), w[ids].to(BF16))
     assert torch.equal(ops.embed_fwd(w, ids, pos=pos, dtype=F32), w[ids] + pos[:50]) and torch.equal(ops.embed_fwd(w, ids, pos=pos), (w[ids] + pos[:50]).to(BF16))
+
+
+def test_the_encoders_embeddings_stay_torchs_and_negative_ids_count_from_the_end():
+    from flash_diffusion_amd import ops
+    from flash_diffusion_amd.clip import MiCLIPTextModel
+    from flash_diffusion_amd.t5 import MiT5EncoderModel
+    torch.manual_seed(0)
+    t5 = MiT5EncoderModel(vocab_size=20, d_model=16, d_kv=8, d_ff=24, num_layers=1, num_heads=2).cuda()
+    clip = MiCLIPTextModel(vocab_size=20, hidden_size=16, intermediate_size=24, num_hidden_layers=1, num_attention_heads=2).cuda()
+    ids = torch.tensor([[3, 19, 0, 18], [1, 2, 19, 5]], device="cuda")
+    back = torch.where(ids > 10, ids - 20, ids)
+    for table in (t5.shared, clip.text_model.embeddings.token_embedding):      # called by itself: fp32, differentiable
+        assert table(ids).dtype == F32 and torch.equal(table(ids), table.weight[ids]) and table(ids).requires_grad
+        assert torch.equal(ops.embed_fwd(table.weight, back, dtype=F32, wrap=True), table.weight[ids])
+        assert bool(torch.isnan(ops.embed_fwd(table.weight, torch.tensor([-21, 20], device="cuda"), wrap=True)).all())
+    assert torch.equal(t5(back.int()).last_hidden_state, t5(ids).last_hidden_state)
+    # (CLIP's pooled row is taken by the largest id, which the negative form changes)
+    assert torch.equal(clip(back).last_hidden_state, clip(ids).last_hidden_state)
