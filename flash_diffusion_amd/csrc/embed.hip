@@ -108,17 +108,22 @@ __device__ __forceinline__ int below_own(const uint32_t* key, uint32_t mine, int
   return r;
 }
 
-__global__ __launch_bounds__(PART) void part_sort_kernel(const void* ids, int ids64, int64_t n, int64_t V, uint32_t* pkey, int32_t* ppos) {
-  __shared__ __attribute__((aligned(16))) uint32_t key[PART];
-  const int64_t p0 = (int64_t)blockIdx.x * PART, p = p0 + threadIdx.x;
+// the place of this thread's key among those of its workgroup of PART (in LDS); threads without one (`real`) keep their own
+__device__ __forceinline__ int rank_in_part(uint32_t* key, uint32_t mine, bool real) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t mine = p < n ? key_of(ids, ids64, V, p) : 0xffffffffu;   // (behind everything; counted nowhere)
   key[threadIdx.x] = mine;
   __syncthreads();
   int r = below_own(key + wave * 64, mine, lane);
   for (int q = 0; q < PART / 64; ++q)
-    if (q != wave) r += below64(key + q * 64, mine + (q < wave && p < n ? 1u : 0u));
-  if (p >= n) r = threadIdx.x;                                            // (the last part's tail keeps its place)
+    if (q != wave) r += below64(key + q * 64, mine + (q < wave && real ? 1u : 0u));
+  return real ? r : threadIdx.x;
+}
+
+__global__ __launch_bounds__(PART) void part_sort_kernel(const void* ids, int ids64, int64_t n, int64_t V, uint32_t* pkey, int32_t* ppos) {
+  __shared__ __attribute__((aligned(16))) uint32_t key[PART];
+  const int64_t p0 = (int64_t)blockIdx.x * PART, p = p0 + threadIdx.x;
+  const uint32_t mine = p < n ? key_of(ids, ids64, V, p) : 0xffffffffu;   // (behind everything; counted nowhere)
+  const int r = rank_in_part(key, mine, p < n);
   pkey[p0 + r] = mine;
   ppos[p0 + r] = (int32_t)p;
 }
@@ -217,18 +222,32 @@ __device__ __forceinline__ void put_row(float* row, int col, int D, const float 
 // The workgroups behind those of the sums write the zeros, the bulk of the bytes: ZROWS rows of the table each, but for the rows of tokens
 // that occur (looked up in the sorted list; each is written once, by its run).
 constexpr int ZROWS = 16;
-template <int VEC>
-__device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const int32_t* sid, int64_t n, int D, float* g, int64_t ldg) {
+// SMALL: at most PART positions and no other launch.  Every workgroup of the sums sorts the ids for itself and follows its runs over the
+// chunk's right edge to their ends, those of the zeros look through the ids (154 positions, 49408 rows of 768: 27 us, with three launches
+// SMALLNOTE).
+template <int VEC, bool SMALL>
+__device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const void* ids, int ids64, const int32_t* sid, int64_t n, int D, float* g, int64_t ldg) {
   const int lane = threadIdx.x & 63;
   const int64_t v = v0 + (lane & (ZROWS - 1));
-  int64_t lo = 0, hi = n;                                     // the first position whose key is not below v
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (sid[mid] < v) lo = mid + 1;
-    else hi = mid;
+  uint32_t todo;
+  if constexpr (SMALL) {
+    __shared__ uint32_t taken;
+    if (threadIdx.x == 0) taken = 0;
+    __syncthreads();
+    const int64_t d = threadIdx.x < n ? id_at(ids, ids64, threadIdx.x) - v0 : -1;
+    if (d >= 0 && d < ZROWS) atomicOr(&taken, 1u << d);
+    __syncthreads();
+    todo = (uint32_t)__ballot(v < V) & ((1u << ZROWS) - 1) & ~taken;
+  } else {
+    int64_t lo = 0, hi = n;                                   // the first position whose key is not below v
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (sid[mid] < v) lo = mid + 1;
+      else hi = mid;
+    }
+    const bool empty = v < V && !(lo < n && sid[lo] == v);
+    todo = (uint32_t)__ballot(empty) & ((1u << ZROWS) - 1);
   }
-  const bool empty = v < V && !(lo < n && sid[lo] == v);
-  uint32_t todo = (uint32_t)__ballot(empty) & ((1u << ZROWS) - 1);
   for (; todo; todo &= todo - 1) {
     float* row = g + (v0 + __ffs(todo) - 1) * ldg;
     for (int c = threadIdx.x * VEC; c < D; c += 256 * VEC) {
@@ -238,11 +257,23 @@ __device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const int32_t* 
   }
 }
 
-template <typename T, int VEC>
-__global__ __launch_bounds__(256, VEC == 8 ? 4 : 5) void run_sum_kernel(const T* dy, int64_t lddy, const int32_t* sid, const int32_t* spos, int64_t n, int D,
-                                                      int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part, int summers,
+template <typename T, int VEC, bool SMALL>
+__global__ __launch_bounds__(256, VEC == 8 || SMALL ? 4 : 5) void run_sum_kernel(const T* dy, int64_t lddy, const void* ids, int ids64, const int32_t* gsid,
+                                                      const int32_t* gspos, int64_t n, int D, int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part, int summers,
                                                       int64_t V) {
-  if ((int)blockIdx.x >= summers) return zero_rows<(VEC > 1 ? 4 : 1)>(((int64_t)blockIdx.x - summers) * ZROWS, V, sid, n, D, g, ldg);
+  if ((int)blockIdx.x >= summers) return zero_rows<(VEC > 1 ? 4 : 1), SMALL>(((int64_t)blockIdx.x - summers) * ZROWS, V, ids, ids64, gsid, n, D, g, ldg);
+  __shared__ __attribute__((aligned(16))) uint32_t key[SMALL ? PART : 4];
+  __shared__ int32_t lsid[SMALL ? PART : 1], lspos[SMALL ? PART : 1];
+  if constexpr (SMALL) {
+    const bool real = threadIdx.x < n;
+    const uint32_t k = real ? key_of(ids, ids64, V, threadIdx.x) : 0xffffffffu;
+    const int r = rank_in_part(key, k, real);
+    lsid[r] = (int32_t)k;
+    lspos[r] = threadIdx.x;
+    __syncthreads();
+  }
+  auto sid = [&](int64_t p) { return SMALL ? lsid[SMALL ? p : 0] : gsid[p]; };
+  auto spos = [&](int64_t p) { return SMALL ? lspos[SMALL ? p : 0] : gspos[p]; };
   __shared__ float head[4][64 * VEC];            // per wave: its share of the run that came in over its left edge
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t c = blockIdx.x / col_groups, p0 = c * CHUNK + wave * ROWS;
@@ -250,15 +281,15 @@ __global__ __launch_bounds__(256, VEC == 8 ? 4 : 5) void run_sum_kernel(const T*
   const int count = (int)(p0 + ROWS < n ? ROWS : p0 < n ? n - p0 : 0);
   int32_t edge[5];                               // the key at each wave's left edge, and behind the chunk
 #pragma unroll
-  for (int q = 0; q < 5; ++q) edge[q] = c * CHUNK + q * ROWS < n ? sid[c * CHUNK + q * ROWS] : -1;
-  const int32_t before = p0 > 0 && count ? sid[p0 - 1] : -1, after = p0 + ROWS < n ? sid[p0 + ROWS] : -1;
+  for (int q = 0; q < 5; ++q) edge[q] = c * CHUNK + q * ROWS < n ? sid(c * CHUNK + q * ROWS) : -1;
+  const int32_t before = p0 > 0 && count ? sid(p0 - 1) : -1, after = p0 + ROWS < n ? sid(p0 + ROWS) : -1;
   float v[ROWS][VEC];
   int32_t id[ROWS];
 #pragma unroll
   for (int q = 0; q < ROWS; ++q) {
     const int64_t p = q < count ? p0 + q : n - 1;
-    id[q] = sid[p];
-    load_cols<T, VEC>(dy + (int64_t)spos[p] * lddy + mine, v[q]);
+    id[q] = sid(p);
+    load_cols<T, VEC>(dy + (int64_t)spos(p) * lddy + mine, v[q]);
   }
   float sum[VEC], out[VEC];
   int32_t leaves = NONE;                         // the run that begins in this wave and leaves it
@@ -294,6 +325,37 @@ __global__ __launch_bounds__(256, VEC == 8 ? 4 : 5) void run_sum_kernel(const T*
 #pragma unroll
         for (int k = 0; k < VEC; ++k) s[k] += head[u][k * 64 + lane];
   };
+  if constexpr (SMALL) {
+    if (leaves != NONE) add_heads(wave + 1, leaves, out);
+    const int64_t e = (c + 1) * CHUNK;           // the run that begins in this chunk and leaves it: summed to its end
+    const bool on = e < n && edge[4] != NONE && sid(e - 1) == edge[4] && (c == 0 || sid(c * CHUNK - 1) != edge[4]);
+    if (on) {
+      float more[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) more[k] = 0.f;
+      for (int64_t p = e + wave * ROWS; p < n && sid(p) == edge[4]; p += CHUNK) {
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) load_cols<T, VEC>(dy + (int64_t)spos(p + q < n ? p + q : n - 1) * lddy + mine, v[q]);
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) {
+          const bool here = p + q < n && sid(p + q) == edge[4];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) more[k] = here ? more[k] + v[q][k] : more[k];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) head[wave][k * 64 + lane] = more[k];
+      __syncthreads();
+      if (leaves == edge[4]) {
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) out[k] += head[u][k * 64 + lane];
+      }
+    }
+    if (leaves != NONE && col < D) put_row<VEC>(g + (int64_t)leaves * ldg, col, D, out, scale, accumulate);
+    return;
+  }
   if (leaves != NONE) {
     add_heads(wave + 1, leaves, out);
     if (col < D) {
@@ -422,7 +484,7 @@ int64_t embed_bwd_ws_bytes(int64_t n, int D) {
 }
 static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
                      int accumulate, float* grad, int64_t ldg, void* ws, hipStream_t st) {
-  const bool parts = n > DIRECT;
+  const bool parts = n > DIRECT, small = n <= PART;
   const int np = cdiv(n, PART);
   int32_t* sid = (int32_t*)ws;
   int32_t* spos = sid + n;
@@ -432,7 +494,7 @@ static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* id
   if (parts) {
     hipLaunchKernelGGL(part_sort_kernel, dim3(np), dim3(PART), 0, st, ids, ids64, n, V, pkey, ppos);
     hipLaunchKernelGGL(order_kernel<true>, dim3(np), dim3(1024), 0, st, ids, ids64, n, V, pkey, ppos, sid, spos);
-  } else if (n > 0) {
+  } else if (!small) {
     hipLaunchKernelGGL(order_kernel<false>, dim3(cdiv(n, 64)), dim3(256), 0, st, ids, ids64, n, V, nullptr, nullptr, sid, spos);
   }
   const bool vec = D >= 8, vec8 = vec && !dy_f32;                                        // (16 bytes of a row per lane)
@@ -441,16 +503,18 @@ static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* id
   FDMI_CHECK(blocks < (1ll << 31), "embed_bwd: too many tokens");
   if (blocks == 0) return 0;
   const dim3 join((unsigned)((chunks + JOINERS - 1) / JOINERS), cdiv(D, vec ? 256 : 64));
-#define EMB_SUM(T, VEC) hipLaunchKernelGGL((run_sum_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)dy, lddy, sid, spos, n, D, \
-                                           groups, scale, accumulate, grad, ldg, part, (int)summers, V)
+#define EMB_SUM(T, VEC) if (small) EMB_SUM_OF(T, VEC, true); else EMB_SUM_OF(T, VEC, false)
+#define EMB_SUM_OF(T, VEC, SMALL) hipLaunchKernelGGL((run_sum_kernel<T, VEC, SMALL>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)dy, lddy, ids, \
+                                           ids64, sid, spos, n, D, groups, scale, accumulate, grad, ldg, part, (int)summers, V)
   if (vec) {
-    if (dy_f32) EMB_SUM(float, 4); else EMB_SUM(bf16_t, 8);
-    if (chunks > 1) hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
+    if (dy_f32) { EMB_SUM(float, 4); } else { EMB_SUM(bf16_t, 8); }
+    if (!small) hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
   } else {
-    if (dy_f32) EMB_SUM(float, 1); else EMB_SUM(bf16_t, 1);
-    if (chunks > 1) hipLaunchKernelGGL(run_join_kernel<1>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
+    if (dy_f32) { EMB_SUM(float, 1); } else { EMB_SUM(bf16_t, 1); }
+    if (!small) hipLaunchKernelGGL(run_join_kernel<1>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
   }
 #undef EMB_SUM
+#undef EMB_SUM_OF
   FDMI_HIP(hipGetLastError());
   return 0;
 }

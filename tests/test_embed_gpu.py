@@ -133,6 +133,24 @@ def test_gradient_where_the_order_is_found_another_way(n):
     assert torch.equal(ops.embed_bwd(dy.cuda(), ids.cuda(), V).cpu(), ref)
 
 
+@pytest.mark.parametrize("kind", ["one", "all", "runs", "padded"])
+@pytest.mark.parametrize("n,D", [(128, 8), (129, 70), (192, 1), (255, 520), (256, 9), (257, 9)])
+def test_gradient_of_short_lists(n, D, kind):
+    ops = _ops()
+    V = 40
+    ids = _ids_of(kind, n, V, n)
+    ids[::37] = torch.tensor([-1, V, 2 ** 31, -(2 ** 40)])[torch.arange(len(ids[::37])) % 4]     # (some outside the table)
+    dy = torch.randint(-3, 4, (n, D), generator=torch.Generator().manual_seed(n))
+    ok = (ids >= 0) & (ids < V)
+    ref = torch.zeros(V, D, dtype=torch.int64).index_add_(0, ids[ok], dy[ok]).float()
+    for dt in (F32, BF16):                                             # (small integers: sums are exact)
+        full = torch.full((V, D), float("nan"), device="cuda")
+        del full
+        assert torch.equal(ops.embed_bwd(dy.to(dt).cuda(), ids.cuda(), V).cpu(), ref)
+        out = torch.ones(V, D, device="cuda")
+        assert torch.equal(ops.embed_bwd(dy.to(dt).cuda(), ids.cuda(), V, out=out).cpu(), ref + 1)
+
+
 @pytest.mark.parametrize("n,it", [(131073, torch.int32), (300000, torch.int64)])
 def test_gradient_of_long_lists(n, it):
     ops = _ops()
