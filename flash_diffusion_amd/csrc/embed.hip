@@ -5,7 +5,7 @@
 //
 // Both are bound by HBM.  The gradient adds in a fixed order (no atomics): positions are ranked by (id, position), a workgroup sums a chunk
 // of the sorted list, and runs of one token that cross a chunk's edge leave partial rows that a last launch adds in order.  Three
-// launches: the ranking, chunk sums together with the zeros, joins (and one before them where the list is long).  16384 bf16 rows of 4096
+// launches: the ranking, chunk sums together with the zeros, joins (one more before them where the list is long, one alone where it is short).  16384 bf16 rows of 4096
 // columns into 32128 fp32 rows, half of them padding: 156 us, 128 of them in the second launch for 725 MB (5.7 TB/s; a copy reaches
 // 4.9, a fill 6.8); 1232 fp32 rows of 768 into 49408: 35 us, 22.5 of them (6.8 TB/s).
 // An id outside the table reads as a row of NaN (a gather cannot raise on the device) and its gradient is dropped.
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t 
 
 // ---- gradient: the order ---------------------------------------------------------------------------------------------------------------
 // A position's place in the list sorted by (id, position) is the number of keys below its own.  Up to DIRECT positions they are counted
-// one by one (quadratic, but one launch: 4.6 us at 256 positions, 7.4 at 1232, 10.1 at 2048, 18 at 4096, 58 at 16384).  Longer lists are
+// one by one (quadratic, but one launch: 4.6 us at 257 positions, 7.4 at 1232, 10.1 at 2048, 18 at 4096, 58 at 16384).  Longer lists are
 // first sorted in parts of 256; the other parts' counts are then binary searches (two launches: 9.1 us at 1232, 9.2 at 2048, 9.7 at 4096,
 // 17.5 at 16384, 98 at 131072; between two launches lies a microsecond).
 // Each part is searched by every other one, so a call of more than SLICE positions (as many parts as run at once) adds up slice after slice:
@@ -223,8 +223,9 @@ __device__ __forceinline__ void put_row(float* row, int col, int D, const float 
 // that occur (looked up in the sorted list; each is written once, by its run).
 constexpr int ZROWS = 16;
 // SMALL: at most PART positions and no other launch.  Every workgroup of the sums sorts the ids for itself and follows its runs over the
-// chunk's right edge to their ends, those of the zeros look through the ids (154 positions, 49408 rows of 768: 27 us, with three launches
-// SMALLNOTE).
+// chunk's right edge to their ends, those of the zeros look through the ids (256 positions: 8.7 us where three launches take 12.7 for 500
+// rows of 256, 21.5 against 28.7 for 49408 of 768; lists of two to eight parts sorted so take longer than with the launches, 17 against 13 us
+// and 63 against 19 for 500 rows, and following a run costs 3 us for 64 positions).
 template <int VEC, bool SMALL>
 __device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const void* ids, int ids64, const int32_t* sid, int64_t n, int D, float* g, int64_t ldg) {
   const int lane = threadIdx.x & 63;
