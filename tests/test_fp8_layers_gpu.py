@@ -322,3 +322,53 @@ def test_the_encoders_embeddings_stay_torchs_and_negative_ids_count_from_the_end
     assert torch.equal(t5(back.int()).last_hidden_state, t5(ids).last_hidden_state)
     # (CLIP's pooled row is taken by the largest id, which the negative form changes)
     assert torch.equal(clip(back).last_hidden_state, clip(ids).last_hidden_state)
+
+
+def _mixed_step(ops, s):
+    n = ops.rmsnorm_fp8(s["x"], None, 1e-6)
+    h = ops.gated_fp8(n, s["w0"], s["w1"])
+    y = ops.gemm_fp8(h, s["wo"], residual=s["x"])
+    return y, ops.gemm_fp8_dgrad(y, s["wo"], out_f32=True), ops.embed_fwd(s["table"], s["ids"]), ops.embed_bwd(y, s["ids"], 300, scale=0.5)
+
+
+def _mixed_state(ops, seed, rows):
+    P = lambda n, k, t=False: ops.pack_weight_fp8((_rand(n, k, seed=seed + n) * k ** -0.5).cuda(), transposed=t)
+    ids = torch.randint(0, 300, (rows,), generator=torch.Generator().manual_seed(seed)).cuda()
+    return dict(x=_rand(rows, 264, seed=seed, dtype=BF16).cuda(), w0=P(520, 264), w1=P(520, 264), wo=P(264, 520, True),
+                table=_rand(300, 264, seed=seed + 1).cuda(), ids=ids)
+
+
+def test_two_streams_at_once():
+    from flash_diffusion_amd import ops
+    states = [_mixed_state(ops, seed, rows) for seed, rows in ((1, 700), (2, 90), (3, 3000))]
+    want = [_mixed_step(ops, s) for s in states]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in states], [[] for _ in states]
+    for _ in range(10):
+        for i, (st, s) in enumerate(zip(streams, states)):
+            with torch.cuda.stream(st):
+                got[i].append(_mixed_step(ops, s))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(a, b) for r in runs for a, b in zip(w, r))
+
+
+def test_two_graphs_of_one_pool_replayed_in_turns():
+    """their scratch lies in one pool: each replay recomputes what it reads"""
+    from flash_diffusion_amd import ops
+    a, b = _mixed_state(ops, 4, 400), _mixed_state(ops, 5, 1500)
+    for s in (a, b):
+        _mixed_step(ops, s)
+    torch.cuda.synchronize()
+    ga, gb = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(ga):
+        ya = _mixed_step(ops, a)
+    with torch.cuda.graph(gb, pool=ga.pool()):
+        yb = _mixed_step(ops, b)
+    for seed in (6, 7, 8):
+        a["x"].copy_(_rand(400, 264, seed=seed))
+        b["x"].copy_(_rand(1500, 264, seed=seed + 9))
+        for g, y, s in ((ga, ya, a), (gb, yb, b), (ga, ya, a)):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(y, _mixed_step(ops, s)))
