@@ -9,6 +9,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import ops
 
@@ -18,12 +19,12 @@ BF16, F32 = torch.bfloat16, torch.float32
 class PackedFp8:
     """The 8-bit form of ONE parameter, packed on first use and again when the parameter has changed (replaced, moved, or written in place:
     torch counts those, but for writes through .data).  It is packed again into the same memory where shape and device allow, so a
-    captured graph that reads it sees the new weight.  The parameter itself is held, so another one at the same address is not taken
-    for it.  Streams other than the one it was packed on wait for the packing; a capture cannot pack (run the layer once before)."""
+    captured graph that reads it sees the new weight.  The parameter itself is held, and its memory by a weak reference, so another one at
+    the same address is not taken for it.  Streams other than the one it was packed on wait for the packing; a capture cannot pack (run the layer once before)."""
 
     def __init__(self, transposed=False):
         self.transposed = transposed
-        self._of = self._key = self._packed = self._event = self._stream = None
+        self._of = self._storage = self._key = self._packed = self._event = self._stream = None
 
     def __deepcopy__(self, memo):
         return PackedFp8(self.transposed)          # (the copy's parameter is another one)
@@ -32,7 +33,8 @@ class PackedFp8:
         return PackedFp8, (self.transposed,)
 
     def __call__(self, w):
-        key = (w._version, w.data_ptr(), w.device, w.dtype, tuple(w.shape))
+        storage = w.untyped_storage()
+        key = (w._version, storage._cdata, w.data_ptr(), w.device, w.dtype, w.shape, w.stride())
         capturing = torch.cuda.is_current_stream_capturing()
         if self._of is not w or self._key != key:
             if capturing:
@@ -45,7 +47,8 @@ class PackedFp8:
             stream, event = torch.cuda.current_stream(), torch.cuda.Event()
             event.record(stream)
             self._packed, self._stream, self._event = packed, stream, event
-            self._key, self._of = key, w
+            # (while the weak reference is held, no other storage can have this one's _cdata)
+            self._key, self._of, self._storage = key, w, StorageWeakRef(storage)
         elif self._event is not None and not capturing:   # (a capture begins with a synchronisation of the device)
             if self._event.query():
                 self._event = None

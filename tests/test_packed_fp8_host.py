@@ -1,0 +1,86 @@
+"""CPU: when fp8.PackedFp8 packs a weight again, and in which order, on stand-ins of the packing and of the device's calls."""
+import pytest
+import torch
+
+from flash_diffusion_amd import fp8, ops
+
+
+class _Packed:
+    """what the stand-in packing returns: a copy of the weight's values"""
+
+    def __init__(self, w, into):
+        self.N, self.K = w.shape
+        self.codes, self.codes_t, self.was = torch.zeros(1), None, w.clone()
+        self.into = into
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """the calls that a PackedFp8 makes, in order"""
+    seen = []
+
+    class Stream:
+        def synchronize(self):
+            seen.append("stream done")
+
+        def wait_event(self, event):
+            seen.append("wait")
+
+    class Event:
+        def record(self, *a):
+            pass
+
+        def query(self):
+            return False
+
+    stream = Stream()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: seen.append("device done"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: stream)
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(ops, "pack_weight_fp8", lambda w, transposed=False, into=None: (seen.append("pack"), _Packed(w, into))[1])
+    return seen
+
+
+def _holds(p, w):
+    got = p(w)
+    return torch.equal(got.was, w.detach()) and p(w) is got
+
+
+def test_a_transposed_data_is_another_weight(calls):
+    w = torch.nn.Parameter(torch.randn(6, 6))
+    p = fp8.PackedFp8()
+    assert _holds(p, w)
+    w.data = w.data.t()                       # the same version, address, type and shape
+    assert _holds(p, w)
+
+
+def test_data_at_the_address_of_data_that_was_freed_is_another_weight(calls):
+    memory = bytearray(4 * 36)                # what an allocator hands out a second time
+
+    def fresh(value):
+        t = torch.frombuffer(memory, dtype=torch.float32).view(6, 6)
+        t.numpy()[:] = value                  # (before the parameter holds it, and not counted as a write to it)
+        return t
+
+    w = torch.nn.Parameter(torch.zeros(6, 6))
+    w.data = fresh(1.0)
+    p = fp8.PackedFp8()
+    assert _holds(p, w)
+    address = w.data_ptr()
+    for value in (2.0, 3.0):
+        w.data = torch.zeros(0)
+        w.data = fresh(value)
+        assert w.data_ptr() == address and _holds(p, w)
+
+
+def test_an_unchanged_weight_is_packed_once_and_a_written_one_again(calls):
+    w = torch.nn.Parameter(torch.randn(5, 7), requires_grad=False)
+    p = fp8.PackedFp8()
+    for _ in range(3):
+        assert _holds(p, w)
+    assert calls.count("pack") == 1
+    w.mul_(2.0)
+    assert _holds(p, w) and calls.count("pack") == 2
+    other = torch.nn.Parameter(w.data, requires_grad=False)          # the same memory behind another parameter
+    assert _holds(p, other) and calls.count("pack") == 3
