@@ -20,11 +20,12 @@ class PackedFp8:
     """The 8-bit form of ONE parameter, packed on first use and again when the parameter has changed (replaced, moved, or written in place:
     torch counts those, but for writes through .data).  It is packed again into the same memory where shape and device allow, so a
     captured graph that reads it sees the new weight.  The parameter itself is held, and its memory by a weak reference, so another one at
-    the same address is not taken for it.  Streams other than the one it was packed on wait for the packing; a capture cannot pack (run the layer once before)."""
+    the same address is not taken for it.  Packing has ended when the call returns (once per weight, the host waits for it): other
+    streams and the replays of captured graphs may read the codes at once.  A capture cannot pack (run the layer once before)."""
 
     def __init__(self, transposed=False):
         self.transposed = transposed
-        self._of = self._storage = self._key = self._packed = self._event = self._stream = None
+        self._of = self._storage = self._key = self._packed = None
 
     def __deepcopy__(self, memo):
         return PackedFp8(self.transposed)          # (the copy's parameter is another one)
@@ -35,25 +36,17 @@ class PackedFp8:
     def __call__(self, w):
         storage = w.untyped_storage()
         key = (w._version, storage._cdata, w.data_ptr(), w.device, w.dtype, w.shape, w.stride())
-        capturing = torch.cuda.is_current_stream_capturing()
         if self._of is not w or self._key != key:
-            if capturing:
+            if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the weight has to be packed before a graph is captured: run the layer once")
             old, into = self._packed, None
             if old is not None:
-                torch.cuda.synchronize()           # (a stream may still read the codes that are overwritten or dropped here)
+                torch.cuda.synchronize(old.codes.device)   # (a stream may still read the codes that are overwritten or dropped here)
                 into = old if (old.N, old.K, old.codes.device) == (*w.shape, w.device) else None
             packed = ops.pack_weight_fp8(w.detach().contiguous(), self.transposed, into)
-            stream, event = torch.cuda.current_stream(), torch.cuda.Event()
-            event.record(stream)
-            self._packed, self._stream, self._event = packed, stream, event
+            torch.cuda.current_stream().synchronize()
             # (while the weak reference is held, no other storage can have this one's _cdata)
-            self._key, self._of, self._storage = key, w, StorageWeakRef(storage)
-        elif self._event is not None and not capturing:   # (a capture begins with a synchronisation of the device)
-            if self._event.query():
-                self._event = None
-            elif torch.cuda.current_stream() != self._stream:
-                torch.cuda.current_stream().wait_event(self._event)
+            self._packed, self._key, self._of, self._storage = packed, key, w, StorageWeakRef(storage)
         return self._packed
 
 

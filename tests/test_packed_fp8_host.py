@@ -23,21 +23,10 @@ def calls(monkeypatch):
         def synchronize(self):
             seen.append("stream done")
 
-        def wait_event(self, event):
-            seen.append("wait")
-
-    class Event:
-        def record(self, *a):
-            pass
-
-        def query(self):
-            return False
-
     stream = Stream()
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: seen.append("device done"))
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: stream)
-    monkeypatch.setattr(torch.cuda, "Event", Event)
     monkeypatch.setattr(ops, "pack_weight_fp8", lambda w, transposed=False, into=None: (seen.append("pack"), _Packed(w, into))[1])
     return seen
 
@@ -84,3 +73,16 @@ def test_an_unchanged_weight_is_packed_once_and_a_written_one_again(calls):
     assert _holds(p, w) and calls.count("pack") == 2
     other = torch.nn.Parameter(w.data, requires_grad=False)          # the same memory behind another parameter
     assert _holds(p, other) and calls.count("pack") == 3
+
+
+def test_packing_has_ended_when_the_call_returns(calls):
+    """what reads the codes next need not ask again: a captured graph replayed on another stream waits for nothing of this one"""
+    w = torch.nn.Parameter(torch.randn(5, 7), requires_grad=False)
+    p = fp8.PackedFp8()
+    first = p(w)
+    assert calls == ["pack", "stream done"] and first.into is None
+    p(w)
+    assert calls == ["pack", "stream done"]
+    w.mul_(2.0)
+    second = p(w)
+    assert calls[2:] == ["device done", "pack", "stream done"] and second.into is first     # (readers before, and behind)
