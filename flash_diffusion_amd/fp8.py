@@ -6,6 +6,8 @@ What trains in front of a frozen 8-bit encoder layer is a token table (textual i
 summed by token.  The weights themselves are frozen: there is no weight gradient.  GPU only; there is no CPU fallback."""
 from __future__ import annotations
 
+import threading
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
@@ -21,10 +23,10 @@ class PackedFp8:
     torch counts those, but for writes through .data).  It is packed again into the same memory where shape and device allow, so a
     captured graph that reads it sees the new weight.  The parameter itself is held, and its memory by a weak reference, so another one at
     the same address is not taken for it.  Packing has ended when the call returns (once per weight, the host waits for it): other
-    streams and the replays of captured graphs may read the codes at once.  A capture cannot pack (run the layer once before)."""
+    streams and the replays of captured graphs may read the codes at once.  A capture cannot pack (run the layer once before).  Threads may share it."""
 
     def __init__(self, transposed=False):
-        self.transposed = transposed
+        self.transposed, self._lock = transposed, threading.Lock()
         self._of = self._storage = self._key = self._packed = None
 
     def __deepcopy__(self, memo):
@@ -34,6 +36,10 @@ class PackedFp8:
         return PackedFp8, (self.transposed,)
 
     def __call__(self, w):
+        with self._lock:
+            return self._of_now(w)
+
+    def _of_now(self, w):
         storage = w.untyped_storage()
         key = (w._version, storage._cdata, w.data_ptr(), w.device, w.dtype, w.shape, w.stride())
         if self._of is not w or self._key != key:

@@ -86,3 +86,25 @@ def test_packing_has_ended_when_the_call_returns(calls):
     w.mul_(2.0)
     second = p(w)
     assert calls[2:] == ["device done", "pack", "stream done"] and second.into is first     # (readers before, and behind)
+
+
+def test_two_threads_pack_a_weight_once(calls, monkeypatch):
+    import threading
+    import time
+    plain = ops.pack_weight_fp8
+    monkeypatch.setattr(ops, "pack_weight_fp8", lambda *a: (time.sleep(0.05), plain(*a))[1])       # (the other thread comes in)
+    w, p = torch.nn.Parameter(torch.randn(5, 7), requires_grad=False), fp8.PackedFp8()
+    for turn in (1, 2):
+        gate, got = threading.Barrier(2), []
+
+        def work():
+            gate.wait()
+            got.append(p(w))
+
+        threads = [threading.Thread(target=work) for _ in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert calls.count("pack") == turn and got[0] is got[1] and torch.equal(got[0].was, w)
+        w.mul_(2.0)
