@@ -56,20 +56,24 @@ class PackedFp8:
         return self._packed
 
 
+def _rows_of(t):
+    """[..., K] as the [M, K] that the products take: rows that are contiguous and do not overlap (a transposed, a broadcast tensor is copied)"""
+    t = t.reshape(-1, t.shape[-1])
+    apart = t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
+    return t if apart and (t.shape[1] <= 1 or t.stride(1) == 1) else t.contiguous()
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, packed, bias, out_f32):
         ctx.packed, ctx.shape, ctx.dtype = packed, x.shape, x.dtype
-        y = ops.gemm_fp8(x.reshape(-1, x.shape[-1]), packed, bias=bias, out_f32=out_f32)
+        y = ops.gemm_fp8(_rows_of(x), packed, bias=bias, out_f32=out_f32)
         return y.view(*x.shape[:-1], packed.N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        dy = dy.reshape(-1, dy.shape[-1])
-        if dy.shape[1] > 1 and dy.stride(1) != 1 or dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]:
-            dy = dy.contiguous()                    # (a broadcast gradient, e.g. that of a sum)
-        dx = ops.gemm_fp8_dgrad(dy, ctx.packed, out_f32=ctx.dtype == F32)
+        dx = ops.gemm_fp8_dgrad(_rows_of(dy), ctx.packed, out_f32=ctx.dtype == F32)
         return dx.view(ctx.shape), None, None, None
 
 

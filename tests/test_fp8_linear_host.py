@@ -1,0 +1,53 @@
+"""CPU: what fp8.Fp8Linear and fp8.TokenEmbedding hand to the products and the lookup, on plain stand-ins of those that keep their checks."""
+import pytest
+import torch
+
+from flash_diffusion_amd import fp8, ops
+
+F32 = torch.float32
+
+
+class _Weight:
+    """a weight in the place of ops.Fp8Weight, and as the buffers that Fp8Linear keeps: its values, and those of its transpose"""
+
+    def __init__(self, w):
+        self.N, self.K = w.shape
+        self.codes = self.scales = self.scales_t = w.detach().clone()
+        self.codes_t = w.detach().t().clone()
+
+
+@pytest.fixture
+def linear(monkeypatch):
+    """a Fp8Linear over plain fp32 products (the checks of their operands are the entry points' own)"""
+    monkeypatch.setattr(ops, "_here", lambda t, what: t)
+    monkeypatch.setattr(ops, "pack_weight_fp8", lambda w, transposed=False: _Weight(w))
+
+    def product(A, W, bias=None, out_f32=False):
+        ops._rows(A, "A")
+        y = A.float() @ W.codes.t()
+        return (y if bias is None else y + bias).to(F32 if out_f32 else torch.bfloat16)
+
+    def dgrad(dY, W, out_f32=False):
+        ops._rows(dY, "dY")
+        return (dY.float() @ W.codes_t.t()).to(F32 if out_f32 else torch.bfloat16)
+
+    monkeypatch.setattr(ops, "gemm_fp8", product)
+    monkeypatch.setattr(ops, "gemm_fp8_dgrad", dgrad)
+    return fp8.Fp8Linear(torch.randn(6, 5, generator=torch.Generator().manual_seed(0)), torch.arange(6.0))
+
+
+INPUTS = {"transposed": lambda x: x.t(), "one row for all": lambda x: x[:, :1].t().expand(7, 5), "one row in a batch": lambda x: x[:, 0].expand(2, 3, 5),
+          "overlapping rows": lambda x: x.reshape(-1).as_strided((9, 5), (2, 1)), "a vector": lambda x: x[:, 2], "every second column": lambda x: x.reshape(-1, 10)[:, ::2],
+          "batch moved": lambda x: x.t().reshape(2, 2, 5).transpose(0, 1), "no rows": lambda x: x.t()[:0], "rows apart": lambda x: x.reshape(-1, 10)[:, :5]}
+
+
+@pytest.mark.parametrize("kind", list(INPUTS))
+def test_linear_takes_inputs_of_any_layout(linear, kind):
+    base = torch.randn(5, 4, generator=torch.Generator().manual_seed(1)).requires_grad_()
+    x = INPUTS[kind](base)
+    w, b = linear.codes, linear.bias
+    y = linear(x)
+    want = torch.nn.functional.linear(x, w, b)
+    assert y.shape == want.shape and torch.allclose(y, want, atol=1e-5)
+    (got,) = torch.autograd.grad(y.sum(), base)
+    assert torch.allclose(got, torch.autograd.grad(want.sum(), base)[0], atol=1e-5)
