@@ -438,6 +438,8 @@ def _rows(t, what, dtypes=(BF16, F32)):
         raise ValueError(f"{what}: need a 2-D tensor of {dtypes}, got {tuple(t.shape)} {t.dtype}")
     M, K = t.shape
     ld, inner = t.stride()
+    if M == 0:
+        return K
     if inner != 1 and K > 1:
         raise ValueError(f"{what}: the last dimension has to be contiguous")
     if M <= 1:
