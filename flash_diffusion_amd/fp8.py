@@ -66,6 +66,7 @@ def _rows_of(t):
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, packed, bias, out_f32):
+        ctx.save_for_backward(packed.codes_t, packed.scales_t)      # (torch then sees a weight that is overwritten before the backward)
         ctx.packed, ctx.shape, ctx.dtype = packed, x.shape, x.dtype
         y = ops.gemm_fp8(_rows_of(x), packed, bias=bias, out_f32=out_f32)
         return y.view(*x.shape[:-1], packed.N)
@@ -73,6 +74,7 @@ class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        ctx.saved_tensors                           # (raises for such a weight)
         dx = ops.gemm_fp8_dgrad(_rows_of(dy), ctx.packed, out_f32=ctx.dtype == F32)
         return dx.view(ctx.shape), None, None, None
 

@@ -51,3 +51,15 @@ def test_linear_takes_inputs_of_any_layout(linear, kind):
     assert y.shape == want.shape and torch.allclose(y, want, atol=1e-5)
     (got,) = torch.autograd.grad(y.sum(), base)
     assert torch.allclose(got, torch.autograd.grad(want.sum(), base)[0], atol=1e-5)
+
+
+def test_a_backward_behind_a_weight_that_was_overwritten_is_refused(linear):
+    """as torch's own layers do: the gradient would be that of another weight than the forward's"""
+    x = torch.randn(3, 5).requires_grad_()
+    y = linear(x)
+    other = {k: v * 2.0 for k, v in linear.state_dict().items()}
+    linear.load_state_dict(other)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    linear(x).sum().backward()
+    assert torch.allclose(x.grad, linear.codes.sum(0).expand(3, 5), atol=1e-5)
