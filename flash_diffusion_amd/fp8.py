@@ -126,7 +126,8 @@ class _LookupFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dw = ops.embed_bwd(dy, ids, ctx.V, scale=ctx.scale).to(ctx.wdtype)
         if ctx.needs_input_grad[1]:                # the position rows are a lookup too, by the last index of ids
-            t = torch.arange(ids.shape[-1] if ids.dim() else 1, dtype=torch.int32, device=ids.device).expand(ids.shape).contiguous()
+            t = torch.arange(ids.shape[-1] if ids.dim() else 1, dtype=torch.int32, device=ids.device)
+            t = t.expand(ids.shape).contiguous() if ids.dim() else t.view(())
             dp = ops.embed_bwd(dy, t, ctx.pos_rows)
         return dw, dp, None, None, None
 

@@ -63,3 +63,29 @@ def test_a_backward_behind_a_weight_that_was_overwritten_is_refused(linear):
         y.sum().backward()
     linear(x).sum().backward()
     assert torch.allclose(x.grad, linear.codes.sum(0).expand(3, 5), atol=1e-5)
+
+
+@pytest.fixture
+def embedding(monkeypatch):
+    """a TokenEmbedding over plain fp32 sums (the gradient's own check of shapes)"""
+    monkeypatch.setattr(ops, "embed_fwd", lambda w, ids, scale=1.0, pos=None, dtype=F32:
+                        (w[ids] * scale + (0.0 if pos is None else pos[:ids.shape[-1] if ids.dim() else 1].view(*ids.shape[-1:], 4))).to(dtype))
+
+    def grad(dy, ids, V, scale=1.0):
+        assert dy.shape[:-1] == ids.shape and ids.is_contiguous()
+        return torch.zeros(V, dy.shape[-1]).index_add_(0, ids.reshape(-1).long(), scale * dy.reshape(ids.numel(), -1))
+
+    monkeypatch.setattr(ops, "embed_bwd", grad)
+    return fp8.TokenEmbedding(9, 4)
+
+
+@pytest.mark.parametrize("shape", [(), (1,), (3,), (2, 3), (2, 0), (2, 1, 3)])
+def test_gradients_of_table_and_positions_for_ids_of_any_shape(embedding, shape):
+    ids = torch.randint(0, 9, shape, generator=torch.Generator().manual_seed(1))
+    pos = torch.randn(5, 4, generator=torch.Generator().manual_seed(2)).requires_grad_()
+    c = torch.randn(*shape, 4, generator=torch.Generator().manual_seed(3))
+    (embedding(ids, scale=0.5, pos=pos, dtype=F32) * c).sum().backward()
+    w, q = embedding.weight.detach().clone().requires_grad_(), pos.detach().clone().requires_grad_()
+    t = torch.arange(shape[-1]) if shape else torch.tensor(0)
+    ((w[ids] * 0.5 + q[t]) * c).sum().backward()
+    assert torch.allclose(embedding.weight.grad, w.grad, atol=1e-6) and torch.allclose(pos.grad, q.grad, atol=1e-6)
