@@ -73,7 +73,7 @@ def embedding(monkeypatch):
 
     def grad(dy, ids, V, scale=1.0):
         assert dy.shape[:-1] == ids.shape and ids.is_contiguous()
-        return torch.zeros(V, dy.shape[-1]).index_add_(0, ids.reshape(-1).long(), scale * dy.reshape(ids.numel(), -1))
+        return torch.zeros(V, dy.shape[-1]).index_add_(0, ids.reshape(-1).long(), scale * dy.reshape(ids.numel(), dy.shape[-1]))
 
     monkeypatch.setattr(ops, "embed_bwd", grad)
     return fp8.TokenEmbedding(9, 4)
