@@ -9,7 +9,7 @@ transformers' state_dict names (``text_model.embeddings.token_embedding.weight``
 Every token-major operation is a launch of libfdmi.so's op-level C-ABI: LayerNorm (affine), bf16 MFMA GEMMs with fused bias /
 residual / activation epilogues (quick-GELU as SiLU(1.702 x) / 1.702 folded into the two MLP GEMMs' alpha, exact GELU as its own
 epilogue), causal self-attention through the exact-f32 materialised-score kernels (77 tokens: the cost is nil), the token and position
-embeddings by the lookup kernel.  torch does the pooled-row selection.  GPU only."""
+embeddings by the lookup kernel.  torch gathers the S position rows (position_ids) and selects the pooled row.  GPU only."""
 from __future__ import annotations
 
 from types import SimpleNamespace
@@ -119,7 +119,7 @@ class MiCLIPTextModel(nn.Module):
         D, H = c.hidden_size, c.num_attention_heads
         emb = tm.embeddings
         dt = self.dt
-        pos = emb.position_embedding.weight[:S].float()
+        pos = emb.position_embedding.weight[emb.position_ids[0, :S]].float().contiguous()      # [S, D]
         hidden: List[torch.Tensor] = []
         if output_hidden_states:               # hidden_states[0] is the embedding in fp32
             h32 = ops.embed_fwd(emb.token_embedding.weight, input_ids, pos=pos, dtype=F32, wrap=True)
