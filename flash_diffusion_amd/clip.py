@@ -118,15 +118,15 @@ class MiCLIPTextModel(nn.Module):
         B, S = input_ids.shape
         D, H = c.hidden_size, c.num_attention_heads
         emb = tm.embeddings
-        dt = self.dt
+        dt, table = self.dt, ops.lookup_table(emb.token_embedding.weight)
         pos = emb.position_embedding.weight[emb.position_ids[0, :S]].float().contiguous()      # [S, D]
         hidden: List[torch.Tensor] = []
         if output_hidden_states:               # hidden_states[0] is the embedding in fp32
-            h32 = ops.embed_fwd(emb.token_embedding.weight, input_ids, pos=pos, dtype=F32, wrap=True)
+            h32 = ops.embed_fwd(table, input_ids, pos=pos, dtype=F32, wrap=True)
             hidden.append(h32)
             h = self._act(h32.view(B * S, D))
         else:
-            h = ops.embed_fwd(emb.token_embedding.weight, input_ids, pos=pos, dtype=dt, wrap=True).view(B * S, D)
+            h = ops.embed_fwd(table, input_ids, pos=pos, dtype=dt, wrap=True).view(B * S, D)
         eps = c.layer_norm_eps
         for lyr in tm.encoder.layers:
             a = lyr.self_attn

@@ -664,6 +664,12 @@ def _ids(ids):
     return ids if ids.is_contiguous() else ids.contiguous()
 
 
+def lookup_table(w):
+    """an embedding's weight as embed_fwd takes it: itself where it is f32 / bf16 with contiguous rows, else a copy (fp32 of other types)"""
+    w = w if w.dtype in (BF16, F32) else w.float()
+    return w if w.stride(-1) == 1 else w.contiguous()
+
+
 def embed_fwd(table, ids, scale=1.0, pos=None, dtype=BF16, wrap=False):
     """scale * table[ids] (+ pos[t], t the last index of ids) -> [*ids.shape, D] in `dtype`: table [V, D] f32 / bf16, ids int32 / int64,
     pos [>= ids.shape[-1], D] f32.  An id outside the table gives a row of NaN; wrap: ids -V .. -1 count from

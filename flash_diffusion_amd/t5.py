@@ -195,7 +195,7 @@ class MiT5EncoderModel(nn.Module):
         assert input_ids.is_cuda, "MiT5EncoderModel runs on the GPU only (no CPU fallback)"
         B, S = input_ids.shape
         D, dt, eps = c.d_model, self.dt, c.layer_norm_epsilon
-        h = ops.embed_fwd(self.shared.weight, input_ids, dtype=dt, wrap=True).view(B * S, D)
+        h = ops.embed_fwd(ops.lookup_table(self.shared.weight), input_ids, dtype=dt, wrap=True).view(B * S, D)
         hidden: List[torch.Tensor] = []
         bias = self._position_bias(S, input_ids.device)
         kbias = None
