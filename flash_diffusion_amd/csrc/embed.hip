@@ -45,9 +45,9 @@ __device__ __forceinline__ void load_cols(const T* p, float v[VEC]) {
 
 // ---- lookup: one wave per token, VEC columns per lane and turn -------------------------------------------------------------------------
 template <typename T, typename O, int VEC>
-__global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n,
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const T* table, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t i0, int64_t n,
                                                         float scale, const float* pos, int64_t pos_rows, int64_t ldp, O* out) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t i = i0 + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= n) return;
   int64_t id = id_at(ids, ids64, i);
   if (ids64 & 2) id += id < 0 ? V : 0;           // counted from the end, as in indexing
@@ -261,8 +261,8 @@ __device__ __forceinline__ void zero_rows(int64_t v0, int64_t V, const void* ids
 template <typename T, int VEC, bool SMALL>
 __global__ __launch_bounds__(256, VEC == 8 || SMALL ? 4 : 5) void run_sum_kernel(const T* dy, int64_t lddy, const void* ids, int ids64, const int32_t* gsid,
                                                       const int32_t* gspos, int64_t n, int D, int col_groups, float scale, int accumulate, float* g, int64_t ldg, float* part, int summers,
-                                                      int64_t V) {
-  if ((int)blockIdx.x >= summers) return zero_rows<(VEC > 1 ? 4 : 1), SMALL>(((int64_t)blockIdx.x - summers) * ZROWS, V, ids, ids64, gsid, n, D, g, ldg);
+                                                      int64_t v0, int64_t V) {
+  if ((int)blockIdx.x >= summers) return zero_rows<(VEC > 1 ? 4 : 1), SMALL>(v0 + ((int64_t)blockIdx.x - summers) * ZROWS, V, ids, ids64, gsid, n, D, g, ldg);
   __shared__ __attribute__((aligned(16))) uint32_t key[SMALL ? PART : 4];
   __shared__ int32_t lsid[SMALL ? PART : 1], lspos[SMALL ? PART : 1];
   if constexpr (SMALL) {
@@ -463,17 +463,19 @@ __global__ __launch_bounds__(JOINERS * 64) void run_join_kernel(const int32_t* s
 int launch_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n, float scale,
                      const float* pos, int64_t pos_rows, int64_t ldp, void* out, int out_f32, hipStream_t st) {
   if (n == 0) return 0;
-  const int64_t blocks = (n + 3) / 4;
-  FDMI_CHECK(blocks < (1ll << 31), "embed_fwd: too many tokens");
   const bool vec = D >= 8;
-#define EMB_FWD(T, O, VEC) hipLaunchKernelGGL((embed_fwd_kernel<T, O, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)table, V, D, ldt, \
-                                              ids, ids64, n, scale, pos, pos_rows, ldp, (O*)out)
-  if (table_f32) { if (out_f32) { if (vec) EMB_FWD(float, float, 8); else EMB_FWD(float, float, 1); }
-                   else { if (vec) EMB_FWD(float, bf16_t, 8); else EMB_FWD(float, bf16_t, 1); } }
-  else { if (out_f32) { if (vec) EMB_FWD(bf16_t, float, 8); else EMB_FWD(bf16_t, float, 1); }
-         else { if (vec) EMB_FWD(bf16_t, bf16_t, 8); else EMB_FWD(bf16_t, bf16_t, 1); } }
+  constexpr int64_t TOKENS = 1ll << 25;            // of one launch (256 threads for four of them)
+  for (int64_t i0 = 0; i0 < n; i0 += TOKENS) {
+    const unsigned blocks = (unsigned)(((n - i0 < TOKENS ? n - i0 : TOKENS) + 3) / 4);
+#define EMB_FWD(T, O, VEC) hipLaunchKernelGGL((embed_fwd_kernel<T, O, VEC>), dim3(blocks), dim3(256), 0, st, (const T*)table, V, D, ldt, \
+                                              ids, ids64, i0, n, scale, pos, pos_rows, ldp, (O*)out)
+    if (table_f32) { if (out_f32) { if (vec) EMB_FWD(float, float, 8); else EMB_FWD(float, float, 1); }
+                     else { if (vec) EMB_FWD(float, bf16_t, 8); else EMB_FWD(float, bf16_t, 1); } }
+    else { if (out_f32) { if (vec) EMB_FWD(bf16_t, float, 8); else EMB_FWD(bf16_t, float, 1); }
+           else { if (vec) EMB_FWD(bf16_t, bf16_t, 8); else EMB_FWD(bf16_t, bf16_t, 1); } }
 #undef EMB_FWD
-  FDMI_HIP(hipGetLastError());
+    FDMI_HIP(hipGetLastError());
+  }
   return 0;
 }
 
@@ -501,12 +503,15 @@ static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* id
   const bool vec = D >= 8, vec8 = vec && !dy_f32;                                        // (16 bytes of a row per lane)
   const int groups = cdiv(D, vec8 ? 512 : vec ? 256 : 64);
   const int64_t chunks = (n + CHUNK - 1) / CHUNK, summers = chunks * groups, blocks = summers + (accumulate ? 0 : (V + ZROWS - 1) / ZROWS);
-  FDMI_CHECK(blocks < (1ll << 31), "embed_bwd: too many tokens");
+  constexpr int64_t MOST = FDMI_LAUNCH_THREADS / 256;       // workgroups of one launch
   if (blocks == 0) return 0;
   const dim3 join((unsigned)((chunks + JOINERS - 1) / JOINERS), cdiv(D, vec ? 256 : 64));
-#define EMB_SUM(T, VEC) if (small) EMB_SUM_OF(T, VEC, true); else EMB_SUM_OF(T, VEC, false)
-#define EMB_SUM_OF(T, VEC, SMALL) hipLaunchKernelGGL((run_sum_kernel<T, VEC, SMALL>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)dy, lddy, ids, \
-                                           ids64, sid, spos, n, D, groups, scale, accumulate, grad, ldg, part, (int)summers, V)
+  // (the zeros of a table of more than about 2^28 rows take a second launch)
+#define EMB_SUM(T, VEC) \
+  for (int64_t b0 = 0; b0 < blocks; b0 += MOST) { if (small) EMB_SUM_OF(T, VEC, true); else EMB_SUM_OF(T, VEC, false); }
+#define EMB_SUM_OF(T, VEC, SMALL) hipLaunchKernelGGL((run_sum_kernel<T, VEC, SMALL>), dim3((unsigned)(blocks - b0 < MOST ? blocks - b0 : MOST)), dim3(256), 0, st, \
+                                           (const T*)dy, lddy, ids, ids64, sid, spos, n, D, groups, scale, accumulate, grad, ldg, part, (int)(b0 ? 0 : summers), \
+                                           b0 ? (b0 - summers) * ZROWS : 0, V)
   if (vec) {
     if (dy_f32) { EMB_SUM(float, 4); } else { EMB_SUM(bf16_t, 8); }
     if (!small) hipLaunchKernelGGL(run_join_kernel<4>, join, dim3(JOINERS * 64), 0, st, sid, n, D, scale, accumulate, grad, ldg, part);
@@ -522,6 +527,8 @@ static int launch_slice(const void* dy, int dy_f32, int64_t lddy, const void* id
 
 int launch_embed_bwd(const void* dy, int dy_f32, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int D, float scale,
                      int accumulate, float* grad, int64_t ldg, void* ws, hipStream_t st) {
+  const int64_t groups = ((int64_t)D + (D < 8 ? 63 : dy_f32 ? 255 : 511)) / (D < 8 ? 64 : dy_f32 ? 256 : 512);
+  FDMI_CHECK(D <= 65535 * 256 && ((n < SLICE ? n : SLICE) + CHUNK - 1) / CHUNK * groups <= FDMI_LAUNCH_THREADS / 256, "embed_bwd: too many columns");
   int64_t at = 0;
   do {
     const int64_t now = n - at < SLICE ? n - at : SLICE;

@@ -2,6 +2,9 @@
 #pragma once
 #include "common.h"
 
+// threads of one launch along a grid's first dimension: HIP refuses 2^32 and more
+constexpr int64_t FDMI_LAUNCH_THREADS = 0xffffffffll;
+
 // One product  C[M][N] = act(X W^T + bias + residual)  of e4m3 codes in tiles (fp8.hip); Kb blocks of 128 along the contraction.  gated:
 // W2 is a second weight of the same form and the result gelu_tanh(X W^T) * (X W2^T) leaves as codes H with scales sh instead of C.
 struct Fp8GemmArgs {

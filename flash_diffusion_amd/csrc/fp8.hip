@@ -652,7 +652,6 @@ int launch_tile(const Fp8GemmArgs& a, hipStream_t st, int row0 = 0, int rows = 0
   constexpr int most = fp8_smem(BM, BN, WM, WN, GATED, SEG);
   static_assert(most <= 160 * 1024, "LDS");
   static std::atomic<uint64_t> allowed;
-  if (const int rc = allow_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>, most, allowed)) return rc;
   const int smem = fp8_smem(BM, BN, WM, WN, GATED, a.Kb);
   const int64_t tilesM = ((int64_t)(rows ? rows : a.M - row0) + BM - 1) / BM, tilesN = ((int64_t)a.N * (GATED ? 2 : 1) + BN - 1) / BN;
   FDMI_CHECK(tilesM * tilesN < (1ll << 30), "gemm_fp8: too many tiles");
@@ -661,6 +660,8 @@ int launch_tile(const Fp8GemmArgs& a, hipStream_t st, int row0 = 0, int rows = 0
   if (fit > 2048 / (WM * WN * 64)) fit = 2048 / (WM * WN * 64);
   const int64_t room = (int64_t)256 * fit, total = tilesM * tilesN;
   const int64_t grid = a.Kb < 2 || total < room ? total : room;
+  FDMI_CHECK(grid * (WM * WN * 64) <= FDMI_LAUNCH_THREADS, "gemm_fp8: too many tiles for one launch");
+  if (const int rc = allow_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>, most, allowed)) return rc;
   hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WM, WN, GATED, WIDE>), dim3((unsigned)grid), dim3(WM * WN * 64), smem, st, a, row0, (int)tilesM,
                      (int)tilesN);
   FDMI_HIP(hipGetLastError());
@@ -794,10 +795,10 @@ int launch_stream(const Fp8GemmArgs& a, hipStream_t st) {
   constexpr int join = fp8_stream_smem(MT, NT), most = std::is_void<RAW>::value ? join : FUSE + FUSE / 128;
   static_assert(join <= most && most <= 160 * 1024, "LDS");
   static std::atomic<uint64_t> allowed;
-  if (const int rc = allow_lds((const void*)fp8_stream_kernel<MT, NT, WIDE, RAW>, most, allowed)) return rc;
   const int codes = std::is_void<RAW>::value ? 0 : a.M * a.Kb * 129, smem = join > codes ? join : codes;
   const int64_t grid = (int64_t)cdiv(a.N, NT * 16) * cdiv(a.M, MT * 16);   // (in one dimension: the second holds 65535)
-  FDMI_CHECK(grid < (1ll << 31), "gemm_fp8: too many tiles");
+  FDMI_CHECK(grid * 512 <= FDMI_LAUNCH_THREADS, "gemm_fp8: too many tiles for one launch");
+  if (const int rc = allow_lds((const void*)fp8_stream_kernel<MT, NT, WIDE, RAW>, most, allowed)) return rc;
   hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, WIDE, RAW>), dim3((unsigned)grid), dim3(512), smem, st, a);
   FDMI_HIP(hipGetLastError());
   return 0;
@@ -809,14 +810,20 @@ int launch_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, f
                      hipStream_t st) {
   if (M == 0) return 0;
   const int Kb = cdiv(K, 128);
-  const int64_t Mp = (M + 15) / 16 * 16, rows4 = (M + 3) / 4;
-  FDMI_CHECK(rows4 < (1ll << 31) && cdiv(Kb, 16) < 65536, "quant_fp8: too many rows or columns");
-  const dim3 grid((unsigned)rows4, norm ? 1 : cdiv(Kb, 16));
-#define FP8_QUANT(T, NORM) hipLaunchKernelGGL((quant_rows_kernel<T, NORM>), grid, dim3(256), 0, st, (const T*)x, ldx, norm, eps, q, s, M, Mp, K, Kb)
-  if (norm) { if (x_f32) FP8_QUANT(float, true); else FP8_QUANT(bf16_t, true); }
-  else { if (x_f32) FP8_QUANT(float, false); else FP8_QUANT(bf16_t, false); }
+  const int64_t Mp = (M + 15) / 16 * 16;
+  FDMI_CHECK(cdiv(Kb, 16) < 65536, "quant_fp8: too many columns");
+  constexpr int64_t SLICE = 1ll << 25;             // rows of one launch (256 threads for four of them)
+  for (int64_t m0 = 0; m0 < M; m0 += SLICE) {
+    const int64_t rows = M - m0 < SLICE ? M - m0 : SLICE;
+    const dim3 grid((unsigned)((rows + 3) / 4), norm ? 1 : cdiv(Kb, 16));
+    const char* from = (const char*)x + m0 * ldx * (x_f32 ? 4 : 2);
+    uint8_t* to = q + m0 * Kb * 128;
+#define FP8_QUANT(T, NORM) hipLaunchKernelGGL((quant_rows_kernel<T, NORM>), grid, dim3(256), 0, st, (const T*)from, ldx, norm, eps, to, s + m0, rows, Mp, K, Kb)
+    if (norm) { if (x_f32) FP8_QUANT(float, true); else FP8_QUANT(bf16_t, true); }
+    else { if (x_f32) FP8_QUANT(float, false); else FP8_QUANT(bf16_t, false); }
 #undef FP8_QUANT
-  FDMI_HIP(hipGetLastError());
+    FDMI_HIP(hipGetLastError());
+  }
   return 0;
 }
 
@@ -841,7 +848,8 @@ double fp8_cost(int64_t M, int64_t N, int Kb, const Fp8Cost& c) {
   return c.fixed + c.tile * w + Kb * (c.block + c.share * w * (tiles < 256 ? 1. - c.idle * (1. - tiles / 256) : 1.));
 }
 double fp8_stream_cost(const Fp8GemmArgs& a, int rows) {   // `rows` rows of X and of W per workgroup
-  const double groups = double((a.M + rows - 1) / rows) * ((a.N + rows - 1) / rows), more = (double)(int64_t)((groups - 1) / 1024);
+  const double groups = double(((int64_t)a.M + rows - 1) / rows) * ((a.N + rows - 1) / rows), more = (double)(int64_t)((groups - 1) / 1024);
+  if (groups * 512 > FDMI_LAUNCH_THREADS) return 1e30;     // (more than one launch holds)
   const double l2 = (groups < 256 ? 256 : groups) * 2 * rows * a.Kb * 128 / 24e6, hbm = double(a.N) * a.Kb * 128 / 4.5e6;
   return (rows == 16 ? 3.5 + .5 * more : 3. + 1.3 * more) + (l2 > hbm ? l2 : hbm);
 }

@@ -227,8 +227,9 @@ int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* cod
  * that size which may be written (not needed where fdmi_fp8_scratch_bytes says 0: a few rows, not gated, are quantised inside the
  * product).  W2 given: the gated form; W and W2 are two weights of one shape and
  * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H, sh (M rows of N columns; the wi_0 / wi_1 pair of a gated feed-forward; no C,
- * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product; M <= 2^30.  C may be the residual (the
- * same rows); it shares no memory with x.                                                                                          */
+ * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product; M <= 2^30 (a product whose tiles
+ * pass 2^32 threads where K <= 128, from 2^36 results on, is refused).  C may be the residual (the same rows); it shares no memory
+ * with x.                                                                                                                          */
 typedef struct fdmi_fp8_desc {
   int32_t M, N, K;
   const void* x; int64_t ldxr; int32_t x_f32;
@@ -249,7 +250,7 @@ int64_t fdmi_fp8_scratch_bytes(int64_t M, int K);   /* of codes and scales toget
  * ids64: bit 0: the ids are int64; bit 1 (lookup only): ids -V .. -1 count from the end of the table, as in indexing.
  * grad[v][:] (+)= scale * sum over ids[i] == v of dy[i][:], fp32 sums in a fixed order (positions ascending in fixed chunks): two
  * runs are bit-identical.  accumulate = 0 writes every row of grad [V][ldg], 1 adds to the rows that occur.  ws: scratch of
- * fdmi_embed_bwd_ws_bytes(n, D) bytes, 16-byte aligned.                                                                              */
+ * fdmi_embed_bwd_ws_bytes(n, D) bytes, 16-byte aligned.  D <= 16776960, and n D below about 2^38 (n counted up to 131072) here.        */
 int fdmi_embed_fwd(const void* table, int table_f32, int64_t V, int D, int64_t ldt, const void* ids, int ids64, int64_t n, float scale,
                    const float* pos, int64_t pos_rows, int64_t ldp, void* out, int out_f32, void* stream);
 int64_t fdmi_embed_bwd_ws_bytes(int64_t n, int D);
