@@ -597,8 +597,8 @@ def _fp8_rows_of(d, A, K, what, gated=False):
 def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what):
     d = Fp8Desc()
     keep = _fp8_rows_of(d, A, K, what)
-    M = d.M
-    if out is None:
+    M, given = d.M, out is not None
+    if not given:
         out = torch.empty((M, N), dtype=F32 if out_f32 else BF16, device=keep.device)
         d.ldc = N
     else:
@@ -607,12 +607,12 @@ def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what
             raise ValueError(f"out: need [{M}, {N}], got {tuple(out.shape)}")
         if not isinstance(A, Fp8Rows) and _overlap(A, out):
             raise ValueError(f"out and {what} share memory")       # (workgroups read A while others already write)
-        if residual is not None and _overlap(residual, out) and (residual.data_ptr(), residual.stride()) != (out.data_ptr(), out.stride()):
-            raise ValueError("out may be the residual, but not share a part of its memory")
     d.N, d.K, d.C, d.out_f32, d.act = N, K, out.data_ptr(), out.dtype == F32, act
     d.W, d.sw = _here(codes, "weight").data_ptr(), scales.data_ptr()
     if bias is not None:
         d.bias = _vector(bias, N, "bias")
+        if given and _overlap(bias.view(1, N), out):
+            raise ValueError("out and bias share memory")
     if residual is not None:
         if act != ACT_NONE:
             raise ValueError("an activation and a residual exclude each other")
@@ -620,6 +620,8 @@ def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what
         if tuple(residual.shape) != (M, N):
             raise ValueError(f"residual: need [{M}, {N}], got {tuple(residual.shape)}")
         d.residual = residual.data_ptr()
+        if given and (d.residual, d.ldr) != (d.C, d.ldc) and _overlap(residual, out):
+            raise ValueError("out may be the residual, but not share a part of its memory")
     if M:
         check(lib().fdmi_gemm_fp8(C.byref(d), _stream()))
     return out

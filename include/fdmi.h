@@ -227,9 +227,9 @@ int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* cod
  * that size which may be written (not needed where fdmi_fp8_scratch_bytes says 0: a few rows, not gated, are quantised inside the
  * product).  W2 given: the gated form; W and W2 are two weights of one shape and
  * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H, sh (M rows of N columns; the wi_0 / wi_1 pair of a gated feed-forward; no C,
- * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product; M <= 2^30 (a product whose tiles
- * pass 2^32 threads where K <= 128, from 2^36 results on, is refused).  C may be the residual (the same rows); it shares no memory
- * with x.                                                                                                                          */
+ * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product; M <= 2^30, and a product of more
+ * than 2^30 tiles (2^24 where K <= 128) of 64 x 64 results or more is refused.  C may be the residual (the same rows); it shares no
+ * memory with x or bias.                                                                                                           */
 typedef struct fdmi_fp8_desc {
   int32_t M, N, K;
   const void* x; int64_t ldxr; int32_t x_f32;
