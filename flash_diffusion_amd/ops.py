@@ -629,21 +629,23 @@ def _fp8_product(A, K, N, codes, scales, bias, residual, act, out, out_f32, what
 
 def gemm_fp8(A, W, *, bias=None, residual=None, act=ACT_NONE, out=None, out_f32=False):
     """act(A W^T + bias) or A W^T + bias + residual with 8-bit operands: A Fp8Rows, or [M, K] bf16 / f32 rows that the call quantises;
-    W Fp8Weight; bias [N] f32; residual and out [M, N] of one type (bf16, or f32 with out_f32); out may be the residual, not A.  fp32 sums, one
-    rounding."""
+    W Fp8Weight; bias [N] f32; residual and out [M, N] of one type (bf16, or f32 with out_f32); out may be the residual, not A.  One rounding
+    to that type.  f32: products and sums in fp32.  bf16: the 8-bit matrix pipe, which drops what lies below 2^-13 of the largest of
+    eight consecutive products and adds such groups in fp32 (include/fdmi.h has the bound); out_f32=True avoids it at half the rate."""
     return _fp8_product(A, W.K, W.N, W.codes, W.scales, bias, residual, act, out, out_f32, "A")
 
 
 def gemm_fp8_dgrad(dY, W, *, residual=None, out=None, out_f32=False):
-    """dY W: the gradient of gemm_fp8's input, dY [M, N] quantised along N.  W has to be packed with transposed=True"""
+    """dY W: the gradient of gemm_fp8's input, dY [M, N] quantised along N; summed as there.  W has to be packed with transposed=True"""
     if W.codes_t is None:
         raise ValueError("gemm_fp8_dgrad needs pack_weight_fp8(w, transposed=True)")
     return _fp8_product(dY, W.N, W.K, W.codes_t, W.scales_t, None, residual, ACT_NONE, out, out_f32, "dY")
 
 
 def gated_fp8(A, W, W2):
-    """gelu_tanh(A W^T) * (A W2^T), quantised: the gated feed-forward's first half (T5: wi_0, wi_1) -> Fp8Rows [M, N].  The product is
-    formed in fp32 and leaves the kernels in no other form than its codes."""
+    """gelu_tanh(A W^T) * (A W2^T), quantised: the gated feed-forward's first half (T5: wi_0, wi_1) -> Fp8Rows [M, N].  Both
+    sums are the 8-bit pipe's (as gemm_fp8's of a bf16 result), their product is formed in fp32 and leaves the kernels in no other form
+    than its codes."""
     if (W.N, W.K) != (W2.N, W2.K):
         raise ValueError(f"the two weights differ in shape: {(W.N, W.K)} and {(W2.N, W2.K)}")
     d = Fp8Desc()
