@@ -5,8 +5,9 @@
 // The scales are powers of two (e8m0 bytes): 2^e is the smallest power with amax <= 448 2^e over the block, so a code never saturates,
 // scaling is exact and the only rounding of the format is the one to e4m3 (round to nearest even).  CDNA4's scaled matrix instruction
 // takes such a scale per lane and 32 contraction steps: a block of 128 hands the same byte to its steps, and the scales cost no
-// arithmetic of their own.  Accumulators are fp32; what the 8-bit pipe adds into them, and which results avoid it: "which matrix pipe" below.  An infinity or NaN of the input becomes the NaN code (e4m3 has no
-// infinity, and a saturated code would hide the overflow) and the block's scale comes from its finite values.
+// arithmetic of their own.  Accumulators are fp32 (what the 8-bit pipe adds into them, and which results avoid it: "which matrix pipe"
+// below).  An infinity or NaN of the input becomes the NaN code (e4m3 has no infinity, and a saturated code would hide the overflow) and
+// the block's scale comes from its finite values.
 //
 // Codes lie in tiles of 16 rows x 64 columns, 1 KiB each: [row tile][column tile][chunk of 16 columns][row][16 bytes].  One wave's load, store or
 // LDS transfer moves whole tiles (row-major codes fill LDS at two thirds of that rate: the first 128 x 128 kernel took 627 us over them for 8192^3
@@ -226,8 +227,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* w, int64_t ldw, int 
 // 2^-10 of each group's largest product, 1e-4 of a typical result, more where large products of one group cancel.  A bf16 result has
 // 1.7e-3 of rounding and takes that pipe; so does the gated product, whose codes have 2^-4 (its feed-forward is 1.70e-3 from 64 bits
 // where fp32 sums are 1.64e-3).  A result that is kept in fp32 takes the bf16 pipe (half the rate; products and sums are fp32; a code times its
-// scale is exact in bf16 for scales from 2^-124 on, its last bits 2^-9 2^-124 being the smallest subnormal; smaller scales, of blocks below
-// 2e-35, round to multiples of 2^-133).
+// scale is exact in bf16 for scales from 2^-124 on, its last bits 2^-9 2^-124 being the smallest subnormal; smaller scales, of blocks up
+// to 1e-35, round to multiples of 2^-133).
 __device__ __forceinline__ mfma_b8 widen8(int lo, int hi, float scale) {   // eight codes times their block's scale, as bf16
   typedef __attribute__((ext_vector_type(2))) __bf16 b2;
   const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);

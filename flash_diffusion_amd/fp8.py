@@ -2,8 +2,9 @@
 gradient flows, ``TokenEmbedding``, ``nn.Embedding``'s lookup and sparse-by-nature gradient on the HIP path, and ``PackedFp8``, the
 cache through which a module keeps the 8-bit form of a parameter (the frozen text encoder of ``t5.py`` with precision="fp8").
 
-What trains in front of a frozen 8-bit encoder layer is a token table (textual inversion): its gradient is the products' input gradient
-summed by token.  The weights themselves are frozen: there is no weight gradient.  GPU only; there is no CPU fallback."""
+A token table trains in front of a chain of frozen ``Fp8Linear`` layers: its gradient is the products' input gradient summed by token.  (The
+text encoders themselves run without gradients.)  The weights are frozen: there is no weight gradient.  GPU only; there is no CPU
+fallback."""
 from __future__ import annotations
 
 import threading
