@@ -6,8 +6,8 @@
 // Both are bound by HBM.  The gradient adds in a fixed order (no atomics): positions are ranked by (id, position), a workgroup sums a chunk
 // of the sorted list, and runs of one token that cross a chunk's edge leave partial rows that a last launch adds in order.  Three
 // launches: the ranking, chunk sums together with the zeros, joins; one more before them where the list is long, one alone where it is
-// short.  16384 bf16 rows of 4096 columns into 32128 fp32 rows, half of them padding: 156 us, 128 of them in the second of these launches
-// for 725 MB (5.7 TB/s; a copy reaches 4.9, a fill 6.8); 1232 fp32 rows of 768 into 49408: 35 us, 22.5 of them (6.8 TB/s).
+// short.  16384 bf16 rows of 4096 columns into 32128 fp32 rows, half of them padding: 156 us, 130 of them in the second of these launches
+// for 725 MB (5.6 TB/s; a copy reaches 4.9, a fill 6.8); 1232 fp32 rows of 768 into 49408: 35 us, 24 of them (6.5 TB/s).
 // An id outside the table reads as a row of NaN (a gather cannot raise on the device) and its gradient is dropped.
 #include "fp8.h"
 

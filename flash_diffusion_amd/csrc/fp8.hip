@@ -839,9 +839,10 @@ int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t
   return 0;
 }
 
-// Which kernel: the least of the times that formulas in the problem's sizes give (microseconds), their constants fitted to times of every kernel on 148
-// problems (16 .. 16384 rows, 64 .. 12288 columns, K 64 .. 10240; half of them drawn, half large).  The chosen one is 4% slower than
-// the best on average (at most 1.6 times, where both are below 3 us).  A tile kernel spends `block` + `share` * w on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU
+// Which kernel: the least of the times that formulas in the problem's sizes give (microseconds), their constants fitted to times of every kernel on drawn
+// problems.  On 148 others (16 .. 16384 rows, 64 .. 12288 columns, K 64 .. 10240, half of them large; every kernel's time for each in
+// profiles/fp8_kernel_choice.csv) the chosen one is 4.5% slower than the best on average for a bf16 result and 5.8% for fp32; by more
+// than 1.4 times in seven of 296, six of them below 5 us and 1588 x 2584 x 3584 in fp32 (69.9 us, 44.7 with 128 x 128 tiles).  A tile kernel spends `block` + `share` * w on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU
 // rounded up; a grid that leaves CUs idle runs its blocks up to `idle` faster.  The streaming kernel is bound by what its workgroups read
 // from L2 (a short grid leaves some CUs idle) or by the weight from memory, and pays for each further turn of 1024 workgroups.
 // For example (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 15.7 / 22.8 / 36, 4.3;  1920 x 4096 x 4096:
@@ -879,6 +880,9 @@ int launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t st) {
                                    {256, 256, .10, 1.39, .2, 7.5, .39}};
   static const Fp8Cost wide[] = {{64, 64, .20, .265, 2., .95, 0.}, {128, 128, .27, .69, 2., 3.25, .37}, {256, 256, .33, 2.74, 0., 9.8, .43}};
   if (a.H) {
+    // A tile is 128 features.  While 128-row ones leave half of the CUs without work, twice as many of 64 rows end sooner (K = 4096: 768 x 2560,
+    // 120 against 240 workgroups, 26.3 and 19.7 us; 120 x 10240, 80 against 160: 25.4 and 18.5), from there on they do not (1024 x 2560, 160 against
+    // 320: 26.9 and 34.6; 200 x 10240: 27.1 and 34.5; profiles/fp8_gated_choice.csv)
     const int64_t cols = ((int64_t)a.N + 127) / 128 * 256;
     if (((int64_t)a.M + 127) / 128 * (cols / 256) < 128) return launch_tile<64, 256, 1, 4, true, false>(a, st);
     const int whole = fp8_whole(a.M, cols), rest = a.M - whole;
