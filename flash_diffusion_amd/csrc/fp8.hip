@@ -840,9 +840,9 @@ int launch_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, uint8_t
 }
 
 // Which kernel: the least of the times that formulas in the problem's sizes give (microseconds), their constants fitted to times of every kernel on drawn
-// problems.  On 148 others (16 .. 16384 rows, 64 .. 12288 columns, K 64 .. 10240, half of them large; every kernel's time for each in
+// problems.  On 147 others (16 .. 16384 rows, 64 .. 12288 columns, K 64 .. 10240, half of them large; every kernel's time for each in
 // profiles/fp8_kernel_choice.csv) the chosen one is 4.5% slower than the best on average for a bf16 result and 5.8% for fp32; by more
-// than 1.4 times in seven of 296, six of them below 5 us and 1588 x 2584 x 3584 in fp32 (69.9 us, 44.7 with 128 x 128 tiles).  A tile kernel spends `block` + `share` * w on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU
+// than 1.4 times in seven of 294, six of them below 5 us and 1588 x 2584 x 3584 in fp32 (69.9 us, 44.7 with 128 x 128 tiles).  A tile kernel spends `block` + `share` * w on a block of 128 and `fixed` + `tile` * w beside, w = tiles per CU
 // rounded up; a grid that leaves CUs idle runs its blocks up to `idle` faster.  The streaming kernel is bound by what its workgroups read
 // from L2 (a short grid leaves some CUs idle) or by the weight from memory, and pays for each further turn of 1024 workgroups.
 // For example (us; 64 / 128 / 128 x 256 / 256 tile, stream): 1 x 4096 x 4096: 11.2 / 15.7 / 22.8 / 36, 4.3;  1920 x 4096 x 4096:
