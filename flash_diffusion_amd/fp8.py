@@ -64,18 +64,23 @@ def _rows_of(t):
     return t if apart and (t.shape[1] <= 1 or t.stride(1) == 1) else t.contiguous()
 
 
+def _versions(packed):
+    """what a write to the weight's transposed codes changes (tensors made in inference mode count no writes)"""
+    return [t._version for t in (packed.codes_t, packed.scales_t) if not t.is_inference()]
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, packed, bias, out_f32):
-        ctx.save_for_backward(packed.codes_t, packed.scales_t)      # (torch then sees a weight that is overwritten before the backward)
-        ctx.packed, ctx.shape, ctx.dtype = packed, x.shape, x.dtype
+        ctx.packed, ctx.versions, ctx.shape, ctx.dtype = packed, _versions(packed), x.shape, x.dtype
         y = ops.gemm_fp8(_rows_of(x), packed, bias=bias, out_f32=out_f32)
         return y.view(*x.shape[:-1], packed.N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        ctx.saved_tensors                           # (raises for such a weight)
+        if _versions(ctx.packed) != ctx.versions:
+            raise RuntimeError("the weight of this Fp8Linear has been modified by an inplace operation since the forward")
         dx = ops.gemm_fp8_dgrad(_rows_of(dy), ctx.packed, out_f32=ctx.dtype == F32)
         return dx.view(ctx.shape), None, None, None
 

@@ -89,3 +89,19 @@ def test_gradients_of_table_and_positions_for_ids_of_any_shape(embedding, shape)
     t = torch.arange(shape[-1]) if shape else torch.tensor(0)
     ((w[ids] * 0.5 + q[t]) * c).sum().backward()
     assert torch.allclose(embedding.weight.grad, w.grad, atol=1e-6) and torch.allclose(pos.grad, q.grad, atol=1e-6)
+
+
+def test_backwards_that_a_frozen_weight_allows(linear):
+    """a second backward needs nothing that the first one frees, and a layer made in inference mode passes gradients on"""
+    x = torch.randn(3, 5).requires_grad_()
+    y = linear(x).sum()
+    y.backward()
+    with torch.inference_mode():
+        made = fp8.Fp8Linear(torch.ones(6, 5))
+    z = torch.randn(3, 5).requires_grad_()
+    made(z).sum().backward()
+    assert torch.equal(z.grad, torch.full((3, 5), 6.0))
+    first = linear(x)
+    g = torch.ones_like(first)
+    a, b = torch.autograd.grad(first, x, g)[0], torch.autograd.grad(first, x, g)[0]
+    assert torch.equal(a, b)
