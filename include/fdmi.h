@@ -223,16 +223,16 @@ int fdmi_quant_fp8(const void* x, int x_f32, int64_t ldx, const float* norm, flo
 int fdmi_pack_fp8(const void* w, int w_f32, int64_t ldw, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t,
                   void* stream);
 /* C[M][N] = act(X W^T + bias) or X W^T + bias + residual, rounded once to C's type (bf16, or fp32 when out_f32; the residual has C's
- * type).  Sums: with out_f32 in fp32, of products in fp32 (codes are widened to bf16, exactly for scales from 2^-124 on, below that to
- * multiples of 2^-133).  Without it, and in the gated form, on the 8-bit matrix pipe: fp32 between groups of eight consecutive columns,
- * but within a group what lies below 2^-13 of its largest product (the power of two in it) is dropped, so a sum is off by up to 2^-10 of
- * the groups' largest products added up: 1e-4 of a typical result, more where large products of one group cancel.  X / sx: codes and scales -- or, when x is given, the unquantised activations x [M][K], and X / sx is scratch of
- * that size which may be written (not needed where fdmi_fp8_scratch_bytes says 0: a few rows, not gated, are quantised inside the
- * product).  W2 given: the gated form; W and W2 are two weights of one shape and
- * gelu_tanh(X W^T) * (X W2^T) leaves quantised as H, sh (M rows of N columns; the wi_0 / wi_1 pair of a gated feed-forward; no C,
- * bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty product; M <= 2^30, and a product of more
- * than 2^30 tiles (2^24 where K <= 128) of 64 x 64 results or more is refused.  C may be the residual (the same rows); it shares no
- * memory with x or bias.                                                                                                           */
+ * type).  X / sx: codes and scales -- or, when x is given, the unquantised activations x [M][K], and X / sx is scratch of that size which
+ * may be written (not needed where fdmi_fp8_scratch_bytes says 0: a few rows, not gated, are quantised inside the product).  W2 given:
+ * the gated form; W and W2 are two weights of one shape and gelu_tanh(X W^T) * (X W2^T) leaves quantised as H, sh (M rows of N columns;
+ * the wi_0 / wi_1 pair of a gated feed-forward; no C, bias, residual or act).  act as in fdmi_gemm (0, 1, 3, 4, 5).  M = 0 is an empty
+ * product; M <= 2^30, and a product of too many tiles for one launch (2^24 of 64 x 64 results where K <= 128) is refused.  C may be the
+ * residual (the same rows); it shares no memory with x or bias.
+ * Sums: with out_f32 in fp32, of products in fp32 (codes are widened to bf16, exactly for scales from 2^-124 on, below that to multiples
+ * of 2^-133).  Without it, and in the gated form, on the 8-bit matrix pipe: fp32 between groups of eight consecutive columns, but within a
+ * group what lies below 2^-13 of its largest product (of the power of two in it) is dropped, so a sum is off by up to 2^-10 of the
+ * groups' largest products added up: 1e-4 of a typical result, more where large products of one group cancel.                       */
 typedef struct fdmi_fp8_desc {
   int32_t M, N, K;
   const void* x; int64_t ldxr; int32_t x_f32;
